@@ -301,6 +301,96 @@ int PARALiA_tile_ddot_noalloc(int dev, void* stream, int64_t N,
                               const double* x, int64_t incx, const double* y, int64_t incy,
                               double* result_dev);
 
+/* ---- mixed-precision linear layer on device-resident data ---------------------------------
+ * Tile calls like the ones above: asynchronous on the caller's stream of GPU `dev`, all
+ * pointers are device pointers of that GPU, PARALiA_tile_status reports a wait that gave up.
+ * They allocate nothing; what scratch they need the caller brings. Two calls that may overlap on
+ * the GPU (two streams, two captured graphs) need scratch of their own each. All of them can be
+ * captured into a graph, after a first call of any tile routine on that GPU has set it up. They
+ * have no counterpart in the reference, whose operations are FP64 and FP32 BLAS. */
+#define PARALIA_F32  0
+#define PARALIA_F16  1
+#define PARALIA_BF16 2
+
+#define PARALIA_ACT_NONE      0
+#define PARALIA_ACT_RELU      1
+#define PARALIA_ACT_GELU      2   /* z * Phi(z), Phi the normal distribution function       */
+#define PARALIA_ACT_GELU_TANH 3   /* z/2 * (1 + tanh(sqrt(2/pi) * (z + 0.044715 z^3)))      */
+#define PARALIA_ACT_SILU      4   /* z / (1 + exp(-z))                                      */
+
+/* Matrix product with bias, activation and residual in its epilogue:
+ *   Z = alpha * op(A) * op(B) + bias,   pre <- Z,   D <- act(Z) + beta * C
+ * with op(A) M x K, op(B) K x N and Z, C, D, pre M x N, column-major, all elements of `type`
+ * (PARALIA_F16 or PARALIA_BF16). `bias` holds M elements, one for each row, or is NULL. `pre`
+ * (NULL: not kept) is what PARALiA_tile_gemm_act_grad reads. Sums are held in FP32; Z and D
+ * are each rounded once from FP32, D from the unrounded Z. As in BLAS, A and B are not read if
+ * alpha or K is 0 and C is not read if beta is 0. D may be C (same leading dimension); otherwise
+ * no output may share memory with an operand. A dense layer on row-major activations x [tokens, in]
+ * and weights w [out, in] is TransA = 'T', A = w, ldA = in, TransB = 'N', B = x, ldB = in,
+ * M = out, N = tokens, K = in, D = y [tokens, out].
+ * Any leading dimension and any address that is a multiple of the element size is accepted;
+ * operands whose address and leading dimension are multiples of 16 bytes are read in place,
+ * others are first copied to scratch. `scratch` is device memory on a 16-byte boundary of at least
+ * PARALiA_tile_gemm_act_scratch_bytes(...) bytes (0 bytes: may be NULL). FP32 operands are
+ * refused with PARALIA_ERR_UNSUPPORTED. */
+int64_t PARALiA_tile_gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N,
+                                            int64_t K, const void* A, int64_t ldA, const void* B,
+                                            int64_t ldB);
+int PARALiA_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB,
+                          int64_t M, int64_t N, int64_t K, float alpha,
+                          const void* A, int64_t ldA, const void* B, int64_t ldB,
+                          const void* bias, int act, float beta, const void* C, int64_t ldC,
+                          void* D, int64_t ldD, void* pre, int64_t ldPre,
+                          void* scratch, int64_t scratch_bytes);
+
+/* Gradient of that product. Given dD, the gradient with respect to D, and `pre` as the forward
+ * call left it (not read for PARALIA_ACT_NONE):
+ *   dZ    = dD . act'(pre)                                  (entry by entry; M x N)
+ *   dbias <- sum over the columns of dZ + betaBias * dbias
+ *   dA    <- alpha * dZ * op(B)^T + betaA * dA              (its transpose if TransA is 'T')
+ *   dB    <- alpha * op(A)^T * dZ + betaB * dB              (its transpose if TransB is 'T')
+ * dA and dB are laid out as A and B are. Each of dA, dB, dbias may be NULL: not computed, and
+ * the operand that only it needs is not read. The gradient with respect to C is beta * dD. A
+ * beta of 1 adds to what earlier calls left (shared weights, several micro-batches). dZ is
+ * rounded to `type` before the two products, which take 16-bit operands; dbias is summed in
+ * FP32 from the unrounded dZ. No gradient may share memory with another or with an operand.
+ * `scratch`: PARALiA_tile_gemm_act_grad_scratch_bytes(...) bytes on a 16-byte boundary. */
+int64_t PARALiA_tile_gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M,
+                                                 int64_t N, int64_t K, const void* A, int64_t ldA,
+                                                 const void* B, int64_t ldB, int act);
+int PARALiA_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char TransB,
+                               int64_t M, int64_t N, int64_t K, float alpha,
+                               const void* A, int64_t ldA, const void* B, int64_t ldB,
+                               int act, const void* pre, int64_t ldPre, const void* dD, int64_t lddD,
+                               float betaA, void* dA, int64_t lddA, float betaB, void* dB, int64_t lddB,
+                               float betaBias, void* dbias, void* scratch, int64_t scratch_bytes);
+
+/* ---- gradient lists -----------------------------------------------------------------------
+ * `count` tensors of n[i] contiguous elements of type[i] (PARALIA_F32, PARALIA_F16 or
+ * PARALIA_BF16, mixed as they come) at device addresses g[i]. The arrays g, n, type, out and
+ * out_type are host memory and are read during the call. Tensors of size 0 are skipped.
+ * `scratch`: device memory of PARALiA_tile_grad_norm_scratch_bytes(count) bytes on an 8-byte
+ * boundary. The order of the sums depends on the list alone, so results are bit-reproducible.
+ *
+ * Global norm: *sumsq <- sum over all elements of g^2, *norm <- its square root (device
+ * memory; either may be NULL). Sums are carried in FP64. */
+int64_t PARALiA_tile_grad_norm_scratch_bytes(int count);
+int PARALiA_tile_grad_norm(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                           const int32_t* type, void* scratch, double* sumsq, float* norm);
+/* Clipping: with norm as above, out[i] <- g[i] * (norm > max_norm ? max_norm / norm : 1), rounded
+ * to out_type[i]. A norm that is not finite clips nothing: the elements are handed on as they are
+ * and *norm tells. out NULL: in place (then nothing is written where the factor is 1). A tensor
+ * that is written may not overlap another of the list; out[i] may be g[i] of the same type.
+ * sumsq and norm may be NULL. */
+int PARALiA_tile_grad_clip(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                           const int32_t* type, void* const* out, const int32_t* out_type,
+                           float max_norm, void* scratch, double* sumsq, float* norm);
+/* The second half of the clipping alone, from a squared norm in device memory: for gradients
+ * that are spread over several GPUs, whose PARALiA_tile_grad_norm sums the caller has added up. */
+int PARALiA_tile_grad_scale(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                            const int32_t* type, void* const* out, const int32_t* out_type,
+                            const double* sumsq, float max_norm, float* norm);
+
 /* ---- memory and input helpers (reference: CoCoMalloc/CoCoFree/CoCoVecInit/CoCoMemcpy,
  * used at dgemm_runner.cpp:55-69,77) ------------------------------------------------- */
 int PARALiA_malloc(void** ptr, int64_t bytes, int loc);   /* loc -1: pinned host     */

@@ -27,6 +27,9 @@ FLAG_KEEP_PINNED = 2
 FLAG_NO_METADATA_REUSE = 4
 FLAG_BETA_ZERO = 8          # autotune_gemm only: model the call with beta == 0
 
+F32, F16, BF16 = 0, 1, 2    # element types of the mixed-precision routines
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
+
 OK = 0
 ERR_INVALID_ARG = 1
 ERR_OUT_OF_MEMORY = 2
@@ -152,6 +155,20 @@ SIGNATURES = {
                                      _dbl, _vp, _i64, _vp]),
     "PARALiA_tile_ddot_noalloc_max_n": (_i64, []),
     "PARALiA_tile_ddot_noalloc": (C.c_int, [C.c_int, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "PARALiA_tile_gemm_act_scratch_bytes": (_i64, [C.c_int, _chr, _chr, _i64, _i64, _i64, _vp, _i64, _vp,
+                                                   _i64]),
+    "PARALiA_tile_gemm_act": (C.c_int, [C.c_int, _vp, C.c_int, _chr, _chr, _i64, _i64, _i64, _flt, _vp, _i64,
+                                        _vp, _i64, _vp, C.c_int, _flt, _vp, _i64, _vp, _i64, _vp, _i64,
+                                        _vp, _i64]),
+    "PARALiA_tile_gemm_act_grad_scratch_bytes": (_i64, [C.c_int, _chr, _chr, _i64, _i64, _i64, _vp, _i64, _vp,
+                                                        _i64, C.c_int]),
+    "PARALiA_tile_gemm_act_grad": (C.c_int, [C.c_int, _vp, C.c_int, _chr, _chr, _i64, _i64, _i64, _flt, _vp,
+                                             _i64, _vp, _i64, C.c_int, _vp, _i64, _vp, _i64, _flt, _vp, _i64,
+                                             _flt, _vp, _i64, _flt, _vp, _vp, _i64]),
+    "PARALiA_tile_grad_norm_scratch_bytes": (_i64, [C.c_int]),
+    "PARALiA_tile_grad_norm": (C.c_int, [C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "PARALiA_tile_grad_clip": (C.c_int, [C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _flt, _vp, _vp, _vp]),
+    "PARALiA_tile_grad_scale": (C.c_int, [C.c_int, _vp, C.c_int, _vp, _vp, _vp, _vp, _vp, _vp, _flt, _vp]),
     "PARALiA_malloc": (C.c_int, [C.POINTER(_vp), _i64, C.c_int]),
     "PARALiA_free": (C.c_int, [_vp, C.c_int]),
     "PARALiA_memcpy": (C.c_int, [_vp, C.c_int, _vp, C.c_int, _i64]),
@@ -417,6 +434,100 @@ def tile_ddot_noalloc(dev, N, x, incx, y, incy, result_dev, stream: int = 0) -> 
     one GPU race on that array. No counterpart in the reference."""
     _check(lib().PARALiA_tile_ddot_noalloc(dev, stream, N, _ptr(x), incx, _ptr(y), incy,
                                            _ptr(result_dev)))
+
+
+def tile_gemm_act_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB) -> int:
+    return int(lib().PARALiA_tile_gemm_act_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _ptr(A), ldA,
+                                                         _ptr(B), ldB))
+
+
+def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, beta, Cm, ldC, D, ldD,
+                  bias=None, act: int = ACT_NONE, pre=None, ldPre: int = 0, scratch=None,
+                  scratch_bytes: int = 0, stream: int = 0) -> None:
+    """``Z = alpha*op(A)*op(B) + bias``, ``pre <- Z``, ``D <- act(Z) + beta*Cm``, FP16 or BF16 (``type``),
+    column-major, on the caller's stream. No counterpart in the reference."""
+    _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _ptr(A), ldA,
+                                       _ptr(B), ldB, _ptr(bias), act, beta, _ptr(Cm), ldC, _ptr(D), ldD,
+                                       _ptr(pre), ldPre, _ptr(scratch), scratch_bytes))
+
+
+def tile_gemm_act_grad_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB, act) -> int:
+    return int(lib().PARALiA_tile_gemm_act_grad_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _ptr(A), ldA,
+                                                              _ptr(B), ldB, act))
+
+
+def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, act, pre, ldPre, dD, lddD,
+                       dA=None, lddA: int = 0, dB=None, lddB: int = 0, dbias=None, betaA: float = 0.0,
+                       betaB: float = 0.0, betaBias: float = 0.0, scratch=None, scratch_bytes: int = 0,
+                       stream: int = 0) -> None:
+    """Gradient of ``tile_gemm_act``: ``dA``, ``dB`` and ``dbias`` (each may be None) from the gradient ``dD``
+    of its result and the pre-activation ``pre`` it kept. No counterpart in the reference."""
+    _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _ptr(A),
+                                            ldA, _ptr(B), ldB, act, _ptr(pre), ldPre, _ptr(dD), lddD, betaA,
+                                            _ptr(dA), lddA, betaB, _ptr(dB), lddB, betaBias, _ptr(dbias),
+                                            _ptr(scratch), scratch_bytes))
+
+
+_TYPE_OF = {"float32": F32, "float16": F16, "bfloat16": BF16}
+
+
+def _type_of(x) -> int:
+    name = str(x.dtype).rsplit(".", 1)[-1]
+    if name not in _TYPE_OF:
+        raise ParaliaError(ERR_INVALID_ARG, f"element type {name} is not float32, float16 or bfloat16")
+    return _TYPE_OF[name]
+
+
+class TensorList:
+    """A list of device tensors as the gradient-list routines take it: addresses, sizes and types
+    of ``tensors``, and of ``out`` where results go elsewhere (None: in place). Built once and
+    used for as long as the tensors stay where they are; it holds references to them."""
+
+    def __init__(self, tensors, out=None):
+        self.tensors = list(tensors)
+        self.out = None if out is None else list(out)
+        if self.out is not None and len(self.out) != len(self.tensors):
+            raise ParaliaError(ERR_INVALID_ARG, f"{len(self.tensors)} tensors, {len(self.out)} outputs")
+        for i, t in enumerate(self.tensors):
+            o = self.out[i] if self.out is not None else t
+            for x in (t, o):
+                if not x.is_contiguous():
+                    raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} is not contiguous")
+                if getattr(x, "is_cuda", True) is False:
+                    raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} is not in GPU memory")
+            if o.numel() != t.numel():
+                raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} has {t.numel()} elements, its output {o.numel()}")
+        n = self.count = len(self.tensors)
+        self.g = (_vp * n)(*[_ptr(t) for t in self.tensors])
+        self.n = (_i64 * n)(*[t.numel() for t in self.tensors])
+        self.type = (_i32 * n)(*[_type_of(t) for t in self.tensors])
+        self.g_out = None if self.out is None else (_vp * n)(*[_ptr(t) for t in self.out])
+        self.out_type = None if self.out is None else (_i32 * n)(*[_type_of(t) for t in self.out])
+
+
+def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
+    return int(lib().PARALiA_tile_grad_norm_scratch_bytes(grads.count))
+
+
+def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
+    """Global norm of a list of tensors: ``norm`` (float32) and ``sumsq`` (float64, its square) are device
+    scalars, either may be None. No counterpart in the reference."""
+    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _ptr(scratch),
+                                        _ptr(sumsq), _ptr(norm)))
+
+
+def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
+    """Global norm of the list, then every tensor times ``max_norm / norm`` where that is below 1, in place or
+    to the list's ``out``. No counterpart in the reference."""
+    _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
+                                        grads.out_type, max_norm, _ptr(scratch), _ptr(sumsq), _ptr(norm)))
+
+
+def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:
+    """The scaling half of ``tile_grad_clip`` from a squared norm in device memory (the sum over several
+    GPUs' lists). No counterpart in the reference."""
+    _check(lib().PARALiA_tile_grad_scale(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
+                                         grads.out_type, _ptr(sumsq), max_norm, _ptr(norm)))
 
 
 def malloc(nbytes: int, loc: int) -> int:

@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 #include <thread>
 #include <string>
 #include <vector>
@@ -242,6 +243,71 @@ int PARALiA_tile_dgemv(int dev, void* stream, char TransA, int64_t M, int64_t N,
   PL_CUDA(launch_dgemv_tile(trans, (int)M, (int)N, alpha, A, ldA, x, incx, beta, y, incy, scratch,
                             static_cast<cudaStream_t>(stream), nullptr));
   return PARALIA_OK;
+}
+
+// ------------------------------ mixed-precision linear layer ------------------------------
+
+int64_t PARALiA_tile_gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N,
+                                            int64_t K, const void* A, int64_t ldA, const void* B,
+                                            int64_t ldB) {
+  return gemm_act_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB);
+}
+
+int PARALiA_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB, int64_t M,
+                          int64_t N, int64_t K, float alpha, const void* A, int64_t ldA,
+                          const void* B, int64_t ldB, const void* bias, int act, float beta,
+                          const void* C, int64_t ldC, void* D, int64_t ldD, void* pre,
+                          int64_t ldPre, void* scratch, int64_t scratch_bytes) {
+  return exec_tile_gemm_act(dev, stream, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, bias,
+                            act, beta, C, ldC, D, ldD, pre, ldPre, scratch, scratch_bytes);
+}
+
+int64_t PARALiA_tile_gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M,
+                                                 int64_t N, int64_t K, const void* A, int64_t ldA,
+                                                 const void* B, int64_t ldB, int act) {
+  return gemm_act_grad_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB, act);
+}
+
+int PARALiA_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char TransB, int64_t M,
+                               int64_t N, int64_t K, float alpha, const void* A, int64_t ldA,
+                               const void* B, int64_t ldB, int act, const void* pre, int64_t ldPre,
+                               const void* dD, int64_t lddD, float betaA, void* dA, int64_t lddA,
+                               float betaB, void* dB, int64_t lddB, float betaBias, void* dbias,
+                               void* scratch, int64_t scratch_bytes) {
+  return exec_tile_gemm_act_grad(dev, stream, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB,
+                                 act, pre, ldPre, dD, lddD, betaA, dA, lddA, betaB, dB, lddB,
+                                 betaBias, dbias, scratch, scratch_bytes);
+}
+
+// ------------------------------ gradient lists ------------------------------
+
+int64_t PARALiA_tile_grad_norm_scratch_bytes(int count) { return grad_norm_scratch_bytes(count); }
+
+// The host side of a list allocates; an exception must not cross the C boundary.
+#define PL_NO_THROW(expr)                                                          \
+  try {                                                                            \
+    return (expr);                                                                 \
+  } catch (const std::exception& ex) {                                             \
+    return fail(PARALIA_ERR_OUT_OF_MEMORY, "host allocation failed: %s", ex.what()); \
+  }
+
+int PARALiA_tile_grad_norm(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                           const int32_t* type, void* scratch, double* sumsq, float* norm) {
+  PL_NO_THROW(exec_tile_grad_norm(dev, stream, count, g, n, type, scratch, sumsq, norm));
+}
+
+int PARALiA_tile_grad_clip(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                           const int32_t* type, void* const* out, const int32_t* out_type,
+                           float max_norm, void* scratch, double* sumsq, float* norm) {
+  PL_NO_THROW(exec_tile_grad_clip(dev, stream, count, g, n, type, out, out_type, max_norm, scratch,
+                                  sumsq, norm));
+}
+
+int PARALiA_tile_grad_scale(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                            const int32_t* type, void* const* out, const int32_t* out_type,
+                            const double* sumsq, float max_norm, float* norm) {
+  PL_NO_THROW(exec_tile_grad_scale(dev, stream, count, g, n, type, out, out_type, sumsq, max_norm,
+                                   norm));
 }
 
 // ------------------------------ memory and inputs ------------------------------

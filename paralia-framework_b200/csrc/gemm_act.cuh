@@ -1,0 +1,46 @@
+// Launchers of the mixed-precision linear-layer kernels (FP16 / BF16 operands, FP32 sums).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace paralia {
+
+// One product with its epilogue:
+//   Z = alpha * op(A) op(B) + bias,  pre <- Z (optional),  D <- act(Z) + beta * C.
+// Every matrix is column-major with 16-bit elements of one type.
+struct GemmActProblem {
+  const void* A;
+  const void* B;
+  const void* bias;    // M elements or null
+  const void* C;       // null when beta == 0
+  void* D;
+  void* pre;           // null when the pre-activation is not kept
+  int64_t ldA, ldB, ldC, ldD, ldPre;
+  int32_t M, N, K;
+  int32_t ta, tb;      // op is the transpose
+  int32_t act;         // PARALIA_ACT_*
+  int32_t bf16;        // 1: BF16, 0: FP16
+  float alpha, beta;
+};
+
+cudaError_t launch_gemm_act(const GemmActProblem& p, cudaStream_t stream);
+
+// dZ <- dD * act'(pre) (dZ may be null; pre is not read for PARALIA_ACT_NONE), and, where
+// dbias is not null, dbias <- row sums of the unrounded product + beta_bias * dbias.
+// `partials` holds act_grad_chunks(M, N) * M floats; it is used when dbias is asked for.
+struct ActGradProblem {
+  const void* pre;
+  const void* dD;
+  void* dZ;
+  void* dbias;
+  float* partials;
+  int64_t ldPre, ldD, ldZ;
+  int32_t M, N;
+  int32_t act, bf16;
+  float beta_bias;
+};
+int act_grad_chunks(int64_t M, int64_t N);
+cudaError_t launch_act_grad(const ActGradProblem& p, cudaStream_t stream);
+
+}  // namespace paralia

@@ -1,0 +1,200 @@
+// Mixed-precision linear-layer routines on device-resident data: argument checks, scratch
+// layout and launches. No counterpart in the reference, whose tile operations are FP64 and
+// FP32 BLAS (Library_scheduler/src/Subkernel.cpp:168,228).
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstring>
+
+#include "exec.hpp"
+#include "gemm_act.cuh"
+#include "runtime.hpp"
+
+namespace paralia {
+namespace {
+
+bool is_trans(char t) { return t == 'T' || t == 't' || t == 'C' || t == 'c'; }
+bool is_flag(char t) { return is_trans(t) || t == 'N' || t == 'n'; }
+
+int64_t round_up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
+
+// What the forward product and its gradient check alike.
+int check_common(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K, float alpha,
+                 int64_t ldA, int64_t ldB, int act) {
+  if (type == PARALIA_F32)
+    return fail(PARALIA_ERR_UNSUPPORTED, "FP32 operands: use PARALiA_tile_sgemm, this routine takes FP16 and BF16");
+  if (type != PARALIA_F16 && type != PARALIA_BF16)
+    return fail(PARALIA_ERR_INVALID_ARG, "element type %d is not PARALIA_F16 or PARALIA_BF16", type);
+  if (!is_flag(TransA) || !is_flag(TransB)) return fail(PARALIA_ERR_INVALID_ARG, "transpose flag is not N or T");
+  if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+    return fail(PARALIA_ERR_INVALID_ARG, "dimension out of range");
+  if (act < PARALIA_ACT_NONE || act > PARALIA_ACT_SILU)
+    return fail(PARALIA_ERR_INVALID_ARG, "activation %d is not one of PARALIA_ACT_*", act);
+  if (ldA < std::max<int64_t>(1, is_trans(TransA) ? K : M) || ldB < std::max<int64_t>(1, is_trans(TransB) ? N : K))
+    return fail(PARALIA_ERR_INVALID_ARG, "leading dimension smaller than the stored row count");
+  if (!std::isfinite(alpha)) return fail(PARALIA_ERR_INVALID_ARG, "alpha is not finite");
+  return PARALIA_OK;
+}
+
+bool odd_address(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
+
+}  // namespace
+
+int64_t gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
+                               const void* A, int64_t ldA, const void* B, int64_t ldB) {
+  (void)type; (void)TransA; (void)TransB; (void)M; (void)N; (void)K; (void)A; (void)ldA; (void)B; (void)ldB;
+  return 0;
+}
+
+int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
+                       int64_t K, float alpha, const void* A, int64_t ldA, const void* B, int64_t ldB,
+                       const void* bias, int act, float beta, const void* C, int64_t ldC, void* D,
+                       int64_t ldD, void* pre, int64_t ldPre, void* scratch, int64_t scratch_bytes) {
+  PL_TRY(check_common(type, TransA, TransB, M, N, K, alpha, ldA, ldB, act));
+  if (!std::isfinite(beta)) return fail(PARALIA_ERR_INVALID_ARG, "beta is not finite");
+  const int64_t rows = std::max<int64_t>(1, M);
+  if (ldD < rows || (beta != 0.0f && ldC < rows) || (pre && ldPre < rows))
+    return fail(PARALIA_ERR_INVALID_ARG, "leading dimension smaller than the stored row count");
+  if (M == 0 || N == 0) return PARALIA_OK;
+  const bool product = K > 0 && alpha != 0.0f;
+  if (!D || (product && (!A || !B)) || (beta != 0.0f && !C)) return fail(PARALIA_ERR_INVALID_ARG, "NULL operand");
+  if (odd_address(A) || odd_address(B) || odd_address(C) || odd_address(D) || odd_address(bias) || odd_address(pre))
+    return fail(PARALIA_ERR_INVALID_ARG, "operand address is not a multiple of the element size");
+  if (D == A || D == B || D == pre || D == bias || (pre && (pre == A || pre == B || pre == bias)) ||
+      (beta != 0.0f && (pre == C || (D == C && ldD != ldC))))
+    return fail(PARALIA_ERR_INVALID_ARG, "an output may share memory with no operand, but D with C at the same leading dimension");
+  DeviceGuard guard;
+  Runtime& rt = Runtime::get();
+  PL_TRY(rt.init());
+  PL_TRY(rt.ensure_device(dev));
+  PL_CUDA(cudaSetDevice(dev));
+  GemmActProblem p;
+  memset(&p, 0, sizeof(p));
+  p.A = A; p.B = B; p.bias = bias; p.C = beta != 0.0f ? C : nullptr; p.D = D; p.pre = pre;
+  p.ldA = ldA; p.ldB = ldB; p.ldC = ldC; p.ldD = ldD; p.ldPre = ldPre;
+  p.M = (int32_t)M; p.N = (int32_t)N; p.K = product ? (int32_t)K : 0;
+  p.ta = is_trans(TransA); p.tb = is_trans(TransB);
+  p.act = act; p.bf16 = type == PARALIA_BF16;
+  p.alpha = alpha; p.beta = beta;
+  (void)scratch; (void)scratch_bytes;
+  PL_CUDA(launch_gemm_act(p, static_cast<cudaStream_t>(stream)));
+  return PARALIA_OK;
+}
+
+namespace {
+
+// Scratch of the gradient: dZ (M x N, leading dimension a multiple of eight), then the
+// partial row sums of the bias gradient.
+struct GradScratch {
+  int64_t ldZ, z_bytes, partial_bytes, total;
+};
+GradScratch grad_scratch(int64_t M, int64_t N) {
+  GradScratch g;
+  g.ldZ = round_up(std::max<int64_t>(1, M), 8);
+  g.z_bytes = round_up(g.ldZ * N * 2, 256);
+  g.partial_bytes = round_up((int64_t)act_grad_chunks(M, N) * M * (int64_t)sizeof(float), 256);
+  g.total = g.z_bytes + g.partial_bytes;
+  return g;
+}
+
+}  // namespace
+
+int64_t gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
+                                    const void* A, int64_t ldA, const void* B, int64_t ldB, int act) {
+  (void)A; (void)B;
+  if (check_common(type, TransA, TransB, M, N, K, 1.0f, ldA, ldB, act) != PARALIA_OK) return 0;
+  return grad_scratch(M, N).total;
+}
+
+int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
+                            int64_t K, float alpha, const void* A, int64_t ldA, const void* B, int64_t ldB,
+                            int act, const void* pre, int64_t ldPre, const void* dD, int64_t lddD,
+                            float betaA, void* dA, int64_t lddA, float betaB, void* dB, int64_t lddB,
+                            float betaBias, void* dbias, void* scratch, int64_t scratch_bytes) {
+  PL_TRY(check_common(type, TransA, TransB, M, N, K, alpha, ldA, ldB, act));
+  if (!std::isfinite(betaA) || !std::isfinite(betaB) || !std::isfinite(betaBias))
+    return fail(PARALIA_ERR_INVALID_ARG, "beta is not finite");
+  const bool ta = is_trans(TransA), tb = is_trans(TransB);
+  const bool uses_pre = act != PARALIA_ACT_NONE;
+  const int64_t rows = std::max<int64_t>(1, M);
+  if (lddD < rows || (uses_pre && ldPre < rows) || (dA && lddA < std::max<int64_t>(1, ta ? K : M)) ||
+      (dB && lddB < std::max<int64_t>(1, tb ? N : K)))
+    return fail(PARALIA_ERR_INVALID_ARG, "leading dimension smaller than the stored row count");
+  const bool want_a = dA && M > 0 && K > 0, want_b = dB && N > 0 && K > 0, want_bias = dbias && M > 0;
+  if (!want_a && !want_b && !want_bias) return PARALIA_OK;
+  const bool entries = M > 0 && N > 0;
+  if (entries && (!dD || (uses_pre && !pre))) return fail(PARALIA_ERR_INVALID_ARG, "NULL operand");
+  if (entries && alpha != 0.0f && ((want_a && !B) || (want_b && !A))) return fail(PARALIA_ERR_INVALID_ARG, "NULL operand");
+  if (odd_address(A) || odd_address(B) || odd_address(pre) || odd_address(dD) || odd_address(dA) ||
+      odd_address(dB) || odd_address(dbias))
+    return fail(PARALIA_ERR_INVALID_ARG, "operand address is not a multiple of the element size");
+  const void* outs[3] = {want_a ? dA : nullptr, want_b ? dB : nullptr, want_bias ? dbias : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    if (!outs[i]) continue;
+    if (outs[i] == A || outs[i] == B || outs[i] == pre || outs[i] == dD || outs[i] == outs[(i + 1) % 3])
+      return fail(PARALIA_ERR_INVALID_ARG, "a gradient may share memory with no operand and no other gradient");
+  }
+  const GradScratch g = grad_scratch(M, N);
+  if (!scratch || scratch_bytes < g.total)
+    return fail(PARALIA_ERR_INVALID_ARG, "the gradient needs %lld bytes of scratch, %lld were given",
+                (long long)g.total, (long long)(scratch ? scratch_bytes : 0));
+  if (reinterpret_cast<uintptr_t>(scratch) & 15)
+    return fail(PARALIA_ERR_INVALID_ARG, "scratch is not aligned to 16 bytes");
+  DeviceGuard guard;
+  Runtime& rt = Runtime::get();
+  PL_TRY(rt.init());
+  PL_TRY(rt.ensure_device(dev));
+  PL_CUDA(cudaSetDevice(dev));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = type == PARALIA_BF16;
+
+  // dZ and the bias gradient in one pass over dD and pre. Without an activation dZ is dD.
+  const bool need_z = entries && uses_pre && (want_a || want_b);
+  char* base = static_cast<char*>(scratch);
+  if (need_z || want_bias) {
+    ActGradProblem a;
+    memset(&a, 0, sizeof(a));
+    a.pre = pre; a.dD = dD; a.dZ = need_z ? base : nullptr; a.dbias = want_bias ? dbias : nullptr;
+    a.partials = reinterpret_cast<float*>(base + g.z_bytes);
+    a.ldPre = ldPre; a.ldD = lddD; a.ldZ = g.ldZ;
+    a.M = (int32_t)M; a.N = (int32_t)N; a.act = act; a.bf16 = bf16; a.beta_bias = betaBias;
+    PL_CUDA(launch_act_grad(a, s));
+  }
+  const void* dZ = need_z ? base : dD;
+  const int64_t ldZ = need_z ? g.ldZ : lddD;
+
+  GemmActProblem p;
+  memset(&p, 0, sizeof(p));
+  p.act = PARALIA_ACT_NONE;
+  p.bf16 = bf16;
+  p.alpha = alpha;
+  if (want_b) {
+    // d op(B) = alpha op(A)^T dZ, stored as B is
+    p.D = dB; p.ldD = lddB; p.C = betaB != 0.0f ? dB : nullptr; p.ldC = lddB; p.beta = betaB;
+    p.K = alpha != 0.0f ? (int32_t)M : 0;
+    if (!tb) {
+      p.A = A; p.ldA = ldA; p.ta = !ta; p.B = dZ; p.ldB = ldZ; p.tb = 0;
+      p.M = (int32_t)K; p.N = (int32_t)N;
+    } else {
+      p.A = dZ; p.ldA = ldZ; p.ta = 1; p.B = A; p.ldB = ldA; p.tb = ta;
+      p.M = (int32_t)N; p.N = (int32_t)K;
+    }
+    PL_CUDA(launch_gemm_act(p, s));
+  }
+  if (want_a) {
+    // d op(A) = alpha dZ op(B)^T, stored as A is
+    p.D = dA; p.ldD = lddA; p.C = betaA != 0.0f ? dA : nullptr; p.ldC = lddA; p.beta = betaA;
+    p.K = alpha != 0.0f ? (int32_t)N : 0;
+    if (!ta) {
+      p.A = dZ; p.ldA = ldZ; p.ta = 0; p.B = B; p.ldB = ldB; p.tb = !tb;
+      p.M = (int32_t)M; p.N = (int32_t)K;
+    } else {
+      p.A = B; p.ldA = ldB; p.ta = tb; p.B = dZ; p.ldB = ldZ; p.tb = 1;
+      p.M = (int32_t)K; p.N = (int32_t)M;
+    }
+    PL_CUDA(launch_gemm_act(p, s));
+  }
+  return PARALIA_OK;
+}
+
+}  // namespace paralia

@@ -1,0 +1,171 @@
+// Host side of the gradient-list routines: argument checks and the description of the list.
+// No counterpart in the reference; they stand beside its level-1 tile operations
+// (Library_scheduler/src/Functions/daxpy.cpp:53-69, ddot.cpp:54-70).
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "exec.hpp"
+#include "grad_list.cuh"
+#include "runtime.hpp"
+
+namespace paralia {
+namespace {
+
+int64_t type_bytes(int t) { return t == PARALIA_F32 ? 4 : (t == PARALIA_F16 || t == PARALIA_BF16) ? 2 : 0; }
+
+struct Range {
+  uintptr_t lo, hi;
+  bool write;
+};
+
+// Refuses memory that is written and also read or written for another tensor: the order of
+// those accesses would decide the result. A tensor scaled in place appears once, as written.
+bool ranges_conflict(std::vector<Range>& r) {
+  auto less = [](const Range& a, const Range& b) { return a.lo < b.lo; };
+  if (!std::is_sorted(r.begin(), r.end(), less)) std::sort(r.begin(), r.end(), less);
+  uintptr_t written = 0, used = 0;   // ends of what lies before, written and at all
+  for (const Range& x : r) {
+    if (x.lo < written || (x.write && x.lo < used)) return true;
+    used = std::max(used, x.hi);
+    if (x.write) written = std::max(written, x.hi);
+  }
+  return false;
+}
+
+// Checks the list and describes its non-empty tensors. out == nullptr: in place.
+int describe(int count, const void* const* g, const int64_t* n, const int32_t* type, void* const* out,
+             const int32_t* out_type, bool writes, std::vector<GradEntry>* entries, GradList* l) {
+  if (count < 0) return fail(PARALIA_ERR_INVALID_ARG, "negative number of tensors");
+  if (count > 0 && (!g || !n || !type)) return fail(PARALIA_ERR_INVALID_ARG, "NULL tensor list");
+  if (out && !out_type) return fail(PARALIA_ERR_INVALID_ARG, "outputs without their element types");
+  int64_t total = 0;
+  for (int i = 0; i < count; ++i) {
+    const int32_t dt = out ? out_type[i] : type[i];
+    if (!type_bytes(type[i]) || !type_bytes(dt))
+      return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: element type is not PARALIA_F32, PARALIA_F16 or PARALIA_BF16", i);
+    if (n[i] < 0 || n[i] > ((int64_t)1 << 48)) return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: size out of range", i);
+    if (n[i] == 0) continue;
+    const void* d = out ? out[i] : g[i];
+    if (!g[i] || !d) return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: NULL pointer", i);
+    if (reinterpret_cast<uintptr_t>(g[i]) % type_bytes(type[i]) || reinterpret_cast<uintptr_t>(d) % type_bytes(dt))
+      return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: address is not a multiple of the element size", i);
+    total += n[i];
+  }
+  l->chunk = grad_chunk_elements(total);
+  l->chunks = 0;
+  entries->reserve(count);
+  std::vector<Range> reads_writes;
+  if (writes) reads_writes.reserve(2 * (size_t)count);
+  for (int i = 0; i < count; ++i) {
+    if (n[i] == 0) continue;
+    GradEntry e;
+    e.src = g[i];
+    e.dst = out ? out[i] : const_cast<void*>(g[i]);
+    e.n = n[i];
+    e.src_type = (uint8_t)type[i];
+    e.dst_type = (uint8_t)(out ? out_type[i] : type[i]);
+    e.flags = 0;
+    e.head = 0;
+    const uintptr_t s = reinterpret_cast<uintptr_t>(e.src), d = reinterpret_cast<uintptr_t>(e.dst);
+    const int64_t sb = type_bytes(e.src_type), db = type_bytes(e.dst_type);
+    if (e.dst == e.src && e.dst_type == e.src_type) e.flags |= GL_IN_PLACE;
+    // the first element from which loads of eight are aligned, and stores too if that can be
+    for (int h = 7; h >= 0; --h)
+      if (((s + h * sb) & 15) == 0) {
+        const uint8_t both = GL_SRC_VEC | (((d + h * db) & 15) == 0 ? GL_DST_VEC : 0);
+        if (both >= (e.flags & (GL_SRC_VEC | GL_DST_VEC))) {
+          e.flags = (uint8_t)((e.flags & GL_IN_PLACE) | both);
+          e.head = (uint8_t)h;
+        }
+      }
+    const int64_t body = std::max<int64_t>(0, e.n - e.head);
+    if (l->chunks > INT32_MAX - body / l->chunk - 1) return fail(PARALIA_ERR_UNSUPPORTED, "the list has too many elements");
+    e.chunk0 = (int32_t)l->chunks;
+    l->chunks += std::max<int64_t>(1, (body + l->chunk - 1) / l->chunk);
+    entries->push_back(e);
+    if (writes) {
+      if (!(e.flags & GL_IN_PLACE)) reads_writes.push_back({s, s + (uintptr_t)(e.n * sb), false});
+      reads_writes.push_back({d, d + (uintptr_t)(e.n * db), true});
+    }
+  }
+  if (writes && ranges_conflict(reads_writes))
+    return fail(PARALIA_ERR_INVALID_ARG, "a tensor to be written overlaps another tensor of the list");
+  l->count = (int)entries->size();
+  l->entries = entries->data();
+  return PARALIA_OK;
+}
+
+int enter(int dev) {
+  Runtime& rt = Runtime::get();
+  PL_TRY(rt.init());
+  PL_TRY(rt.ensure_device(dev));
+  PL_CUDA(cudaSetDevice(dev));
+  return PARALIA_OK;
+}
+
+int check_max_norm(float max_norm) {
+  if (!(max_norm >= 0.0f)) return fail(PARALIA_ERR_INVALID_ARG, "max_norm is negative or not a number");
+  return PARALIA_OK;
+}
+
+int check_scratch(const void* scratch) {
+  if (!scratch) return fail(PARALIA_ERR_INVALID_ARG, "NULL scratch");
+  if (reinterpret_cast<uintptr_t>(scratch) & 7) return fail(PARALIA_ERR_INVALID_ARG, "scratch is not aligned to 8 bytes");
+  return PARALIA_OK;
+}
+
+}  // namespace
+
+int64_t grad_norm_scratch_bytes(int count) {
+  return grad_partials(std::max(count, 0)) * (int64_t)sizeof(double);
+}
+
+int exec_tile_grad_norm(int dev, void* stream, int count, const void* const* g, const int64_t* n, const int32_t* type,
+                        void* scratch, double* sumsq, float* norm) {
+  std::vector<GradEntry> entries;
+  GradList l;
+  PL_TRY(describe(count, g, n, type, nullptr, nullptr, false, &entries, &l));
+  PL_TRY(check_scratch(scratch));
+  if (!sumsq && !norm) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq and norm");
+  DeviceGuard guard;
+  PL_TRY(enter(dev));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int used = 0;
+  PL_CUDA(launch_grad_sumsq(l, static_cast<double*>(scratch), &used, s));
+  PL_CUDA(launch_grad_norm_final(static_cast<double*>(scratch), used, sumsq, norm, s));
+  return PARALIA_OK;
+}
+
+int exec_tile_grad_clip(int dev, void* stream, int count, const void* const* g, const int64_t* n, const int32_t* type,
+                        void* const* out, const int32_t* out_type, float max_norm, void* scratch, double* sumsq,
+                        float* norm) {
+  std::vector<GradEntry> entries;
+  GradList l;
+  PL_TRY(check_max_norm(max_norm));
+  PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
+  PL_TRY(check_scratch(scratch));
+  DeviceGuard guard;
+  PL_TRY(enter(dev));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int used = 0;
+  PL_CUDA(launch_grad_sumsq(l, static_cast<double*>(scratch), &used, s));
+  PL_CUDA(launch_grad_scale(l, static_cast<double*>(scratch), used, max_norm, sumsq, norm, s));
+  return PARALIA_OK;
+}
+
+int exec_tile_grad_scale(int dev, void* stream, int count, const void* const* g, const int64_t* n,
+                         const int32_t* type, void* const* out, const int32_t* out_type, const double* sumsq,
+                         float max_norm, float* norm) {
+  std::vector<GradEntry> entries;
+  GradList l;
+  PL_TRY(check_max_norm(max_norm));
+  PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
+  if (!sumsq) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq");
+  DeviceGuard guard;
+  PL_TRY(enter(dev));
+  PL_CUDA(launch_grad_scale(l, sumsq, 1, max_norm, nullptr, norm, static_cast<cudaStream_t>(stream)));
+  return PARALIA_OK;
+}
+
+}  // namespace paralia
