@@ -1,68 +1,570 @@
-// Matrix product with bias, activation and residual in its epilogue, FP16 / BF16.
+// Matrix product with bias, activation and residual in its epilogue, FP16 / BF16:
+//   Z = alpha * op(A) op(B) + bias,  pre <- Z,  D <- act(Z) + beta * C,   column-major,
+// on the fifth-generation tensor cores, and the elementwise part of its gradient.
+//
+// The product as the tensor core sees it is acc[r, q] = sum_k X[r, k] Y[q, k]: r runs over the
+// lanes of tensor memory (the MMA's M), q over its columns (the MMA's N). QC chooses which
+// dimension of D lies on the columns:
+//   QC = true   r = column of D, q = row of D: a thread holds a run of one column of D, which is
+//               contiguous, and moves it 16 bytes at a time. For D with many rows and columns.
+//   QC = false  r = row of D, q = column of D: neighbouring lanes hold neighbouring rows, so every
+//               access of a warp is 64 contiguous bytes at any alignment. For few columns (a
+//               token or a small batch: the MMA's N is as small as 16) and for unaligned D.
+//
+// Operand tiles are 64 k deep and come by TMA with 128-byte swizzle, in the storage order the
+// operand has (idesc and descriptors tell the tensor core whether k or r / q is contiguous), so
+// all four transpose combinations run without a repacking pass:
+//   k contiguous        one box of 64 k x rows; eight rows of 128 bytes are one swizzle atom
+//                       (stride byte offset 1024), 16 k further is 32 bytes further.
+//   r / q contiguous    boxes of 64 rows x 64 k; eight k of 128 bytes are one atom (stride byte
+//                       offset 1024), the next 64 rows are 8 KB away (leading byte offset), 16 k
+//                       further is 2 KB further.
+// TMA fills with zeros outside the matrix, so no size has to be a multiple of anything.
+//
+// Roles: warp 0 loads, warp 1 issues MMAs, the others are the epilogue, with two accumulators in
+// tensor memory so that the epilogue of one tile runs under the MMAs of the next. CG = 2 pairs
+// two CTAs on one 256 x BN tile: each loads its half of X and of Y, the leader issues the MMAs
+// for both. Every wait is bounded; on a timeout the CTA records an error word, stops issuing
+// work and exits.
+//
+// Split k: with few tiles, the S CTAs of a cluster take a run of k each, put their FP32
+// accumulators into their shared memory and each sums one S-th of the columns over the cluster
+// through distributed shared memory, in rank order: one launch, no scratch, the same bits every
+// time.
 #include "gemm_act.cuh"
 
 #include <algorithm>
+#include <atomic>
+#include <cstring>
 
 #include "act_math.cuh"
+#include "runtime.hpp"
+#include "sm100_prims.cuh"
 
 namespace paralia {
+using namespace prims;
+
 namespace {
 
-constexpr int GA_TILE = 64;
-constexpr int GA_K = 16;
+constexpr int GA_BK = 64;              // k per stage: 128 bytes, one swizzle row
+constexpr int GA_MAX_STAGES = 12;
+constexpr int GA_X_BYTES = 128 * GA_BK * 2;
+constexpr int GA_PANEL = 8;            // q tiles per panel of the tile numbering
 
-// 64 x 64 tile of D per block of 256 threads, 4 x 4 entries per thread, operands through
-// shared memory as FP32.
-__global__ void __launch_bounds__(256) gemm_act_kernel(const GemmActProblem p) {
-  __shared__ float sa[GA_K][GA_TILE + 1], sb[GA_K][GA_TILE + 1];
-  const int m0 = blockIdx.x * GA_TILE, n0 = blockIdx.y * GA_TILE;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const bool bf = p.bf16 != 0;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < p.K; k0 += GA_K) {
-    for (int i = threadIdx.x; i < GA_TILE * GA_K; i += 256) {
-      // walk the contiguous dimension of the stored operand first
-      const int ka = p.ta ? i % GA_K : i / GA_TILE, ma = p.ta ? i / GA_K : i % GA_TILE;
-      const int kb = p.tb ? i / GA_TILE : i % GA_K, nb = p.tb ? i % GA_TILE : i / GA_K;
-      const int64_t m = m0 + ma, n = n0 + nb;
-      sa[ka][ma] = (m < p.M && k0 + ka < p.K)
-                       ? load16(p.A, p.ta ? (k0 + ka) + m * p.ldA : m + (int64_t)(k0 + ka) * p.ldA, bf)
-                       : 0.0f;
-      sb[kb][nb] = (n < p.N && k0 + kb < p.K)
-                       ? load16(p.B, p.tb ? n + (int64_t)(k0 + kb) * p.ldB : (k0 + kb) + n * p.ldB, bf)
-                       : 0.0f;
-    }
-    __syncthreads();
+struct GemmActKernelArgs {
+  const void* bias;
+  const void* C;
+  void* D;
+  void* pre;
+  int64_t ldC, ldD, ldPre;
+  int64_t tiles;
+  int32_t M, N;
+  int32_t r_tiles, q_tiles;
+  int32_t kblocks;
+  int32_t stages, stage_bytes;   // per CTA
+  int32_t split;                 // CTAs that share a tile's k (the cluster, CG == 1)
+  int32_t x_mn, y_mn;            // 1: r / q contiguous, 0: k contiguous
+  int32_t act, bf16;
+  int32_t vec;                   // D, C, pre and bias allow 16-byte accesses along M
+  float alpha, beta;
+  int* status;
+};
+
+template <int BN>
+struct GaShape {
+  static constexpr int EPILOGUE_WARPS = BN >= 128 ? 8 : 4;
+  static constexpr int THREADS = 64 + 32 * EPILOGUE_WARPS;
+};
+
+struct GaCtl {
+  uint64_t full[GA_MAX_STAGES];
+  uint64_t empty[GA_MAX_STAGES];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+constexpr int GA_CTL_BYTES = 256;
+static_assert(sizeof(GaCtl) <= GA_CTL_BYTES, "control block");
+
+// ------------------------------------------------------------------ instructions
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Tiled TMA load without multicast; `bar` is a shared::cluster address. With CG == 2 it may lie in
+// the other CTA of the pair.
+template <int CG>
+__device__ __forceinline__ void ga_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  if (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(0)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(0)
+        : "memory");
+}
+
+// Shared-memory operand descriptor with 128-byte swizzle.
+__device__ __forceinline__ uint64_t ga_desc(uint32_t saddr, int mn_major) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(mn_major ? (8192 >> 4) : 1) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <int CG>
+__device__ __forceinline__ void ga_mma(uint32_t tmem_d, uint64_t xdesc, uint64_t ydesc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(xdesc), "l"(ydesc),
+        "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), "l"(xdesc), "l"(ydesc),
+        "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrive at `bar` (in both CTAs of the pair with CG == 2) when the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void ga_commit(uint64_t* bar) {
+  if (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+
+__device__ __forceinline__ void ga_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void ga_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+template <int W>
+__device__ __forceinline__ void ga_tmem_ld(uint32_t taddr, float (&v)[W]);
+template <>
+__device__ __forceinline__ void ga_tmem_ld<32>(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < GA_K; ++k) {
-      float a[4], b[4];
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+template <>
+__device__ __forceinline__ void ga_tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = sa[k][tx + 16 * i];
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// ------------------------------------------------------------------ epilogue
+// Eight neighbouring rows m .. m+7 of column n of D (QC): acc -> D, pre.
+template <int ACT>
+__device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m, int64_t n, float* v) {
+  const bool bf = a.bf16 != 0;
+  if (a.vec && m + 8 <= a.M) {
+    uint4 c = make_uint4(0, 0, 0, 0), b = make_uint4(0, 0, 0, 0);
+    if (a.C) c = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.C) + m + n * a.ldC);
+    if (a.bias) b = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.bias) + m));
+    const uint32_t cv[4] = {c.x, c.y, c.z, c.w}, bv[4] = {b.x, b.y, b.z, b.w};
+    uint32_t z[4], d[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = sb[k][ty + 16 * j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-  with_act(p.act, [&](auto a) {
     for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + tx + 16 * i;
-      if (m >= p.M) continue;
-      const float bias = p.bias ? load16(p.bias, m, bf) : 0.0f;
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + ty + 16 * j;
-        if (n >= p.N) continue;
-        const float z = fmaf(p.alpha, acc[i][j], bias);
-        if (p.pre) store16(p.pre, m + n * p.ldPre, z, bf);
-        float v = act_value<decltype(a)::value>(z);
-        if (p.C) v = fmaf(p.beta, load16(p.C, m + n * p.ldC, bf), v);
-        store16(p.D, m + n * p.ldD, v, bf);
+      const float2 bb = unpack16(bv[i], bf), cc = unpack16(cv[i], bf);
+      const float z0 = fmaf(a.alpha, v[2 * i], bb.x), z1 = fmaf(a.alpha, v[2 * i + 1], bb.y);
+      z[i] = pack16(z0, z1, bf);
+      float d0 = act_value<ACT>(z0), d1 = act_value<ACT>(z1);
+      if (a.C) {
+        d0 = fmaf(a.beta, cc.x, d0);
+        d1 = fmaf(a.beta, cc.y, d1);
+      }
+      d[i] = pack16(d0, d1, bf);
+    }
+    if (a.pre) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.pre) + m + n * a.ldPre) = make_uint4(z[0], z[1], z[2], z[3]);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.D) + m + n * a.ldD) = make_uint4(d[0], d[1], d[2], d[3]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (m + i >= a.M) break;
+    const float z = fmaf(a.alpha, v[i], a.bias ? load16(a.bias, m + i, bf) : 0.0f);
+    if (a.pre) store16(a.pre, m + i + n * a.ldPre, z, bf);
+    float d = act_value<ACT>(z);
+    if (a.C) d = fmaf(a.beta, load16(a.C, m + i + n * a.ldC, bf), d);
+    store16(a.D, m + i + n * a.ldD, d, bf);
+  }
+}
+
+// W accumulator columns q0 .. q0+W-1 of lane row r.
+template <bool QC, int W>
+__device__ __forceinline__ void ga_finish(const GemmActKernelArgs& a, int64_t r, int64_t q0, float (&v)[W]) {
+  with_act(a.act, [&](auto t) {
+    constexpr int ACT = decltype(t)::value;
+    if constexpr (QC) {
+      if (r >= a.N) return;
+#pragma unroll
+      for (int g = 0; g < W / 8; ++g)
+        if (q0 + 8 * g < a.M) ga_finish8<ACT>(a, q0 + 8 * g, r, &v[8 * g]);
+    } else {
+      if (r >= a.M) return;
+      const bool bf = a.bf16 != 0;
+      const float b = a.bias ? load16(a.bias, r, bf) : 0.0f;
+      float c[W];
+      if (a.C) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) c[j] = q0 + j < a.N ? load16(a.C, r + (q0 + j) * a.ldC, bf) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        if (q0 + j >= a.N) break;
+        const float z = fmaf(a.alpha, v[j], b);
+        if (a.pre) store16(a.pre, r + (q0 + j) * a.ldPre, z, bf);
+        float d = act_value<ACT>(z);
+        if (a.C) d = fmaf(a.beta, c[j], d);
+        store16(a.D, r + (q0 + j) * a.ldD, d, bf);
       }
     }
   });
+}
+
+// ------------------------------------------------------------------ kernel
+struct GaTile {
+  int rt, qt;
+};
+// Tiles are numbered in panels of GA_PANEL q tiles, inside a panel along q first: what runs at
+// one time then shares few X and few Y tiles, which cuts what is pulled through L2.
+__device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int64_t tile) {
+  const int64_t per_panel = (int64_t)a.r_tiles * GA_PANEL;
+  const int panel = (int)(tile / per_panel);
+  const int width = min(GA_PANEL, a.q_tiles - panel * GA_PANEL);
+  const int64_t rest = tile - panel * per_panel;
+  GaTile t;
+  t.rt = (int)(rest / width);
+  t.qt = panel * GA_PANEL + (int)(rest % width);
+  return t;
+}
+
+template <int BN, int CG, bool QC>
+__global__ void __launch_bounds__(GaShape<BN>::THREADS, 1)
+gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                const __grid_constant__ GemmActKernelArgs a) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ GaCtl ctl_mem;
+  GaCtl* ctl = &ctl_mem;
+  volatile int* abort_flag = &ctl->abort_flag;
+  constexpr int EW = GaShape<BN>::EPILOGUE_WARPS;
+  constexpr int YROWS = BN / CG;                       // rows of Y this CTA loads
+  constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = (CG == 2 || a.split > 1) ? cluster_rank() : 0;
+  const int split = CG == 1 ? a.split : 1;
+  const int group = CG * split;                        // CTAs that share a tile
+  const int64_t first_tile = blockIdx.x / group, tile_step = gridDim.x / group;
+  // this CTA's run of k blocks
+  const int kb0 = split > 1 ? (int)((int64_t)a.kblocks * rank / split) : 0;
+  const int kb1 = split > 1 ? (int)((int64_t)a.kblocks * (rank + 1) / split) : a.kblocks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(&ctl->full[s], 1);
+      mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&ctl->acc_full[b], 1);
+      mbar_init(&ctl->acc_empty[b], EW * CG);
+    }
+    ctl->abort_flag = 0;
+    ctl->tmem_base = 0;
+    mbar_fence_init();
+    prefetch_tensormap(&map_x);
+    prefetch_tensormap(&map_y);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    if (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)),
+                   "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl->tmem_base)),
+                   "r"(TMEM_COLS)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+  }
+  ga_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();     // the other CTA's barriers are initialised, its columns allocated
+  ga_fence_after();
+  const uint32_t tmem_base = ctl->tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------ producer ------------------------------
+    if (lane == 0) {
+      int64_t it = 0;
+      bool ok = true;
+      for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+        const GaTile t = ga_tile(a, tile);
+        const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
+        const int q0 = t.qt * BN + (CG == 2 ? (int)rank * YROWS : 0);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = (int)(it % a.stages);
+          const int64_t use = it / a.stages;
+          if (use > 0 && !mbar_wait_bounded(&ctl->empty[s], (uint32_t)((use - 1) & 1), abort_flag)) {
+            if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_EMPTY_WAIT_TIMEOUT); }
+            ok = false;
+            break;
+          }
+          const uint32_t x = smem_u32(smem) + s * a.stage_bytes, y = x + GA_X_BYTES;
+          uint32_t bar = smem_u32(&ctl->full[s]);
+          if (CG == 2) bar = map_rank(bar, 0);
+          if (CG == 1 || rank == 0) mbar_expect_tx(&ctl->full[s], a.stage_bytes * CG);
+          if (a.x_mn) {
+            ga_load<CG>(x, &map_x, bar, r0, kb * GA_BK);
+            ga_load<CG>(x + 8192, &map_x, bar, r0 + 64, kb * GA_BK);
+          } else {
+            ga_load<CG>(x, &map_x, bar, kb * GA_BK, r0);
+          }
+          if (a.y_mn) {
+#pragma unroll
+            for (int j = 0; j < (YROWS + 63) / 64; ++j) ga_load<CG>(y + j * 8192, &map_y, bar, q0 + j * 64, kb * GA_BK);
+          } else {
+            ga_load<CG>(y, &map_y, bar, kb * GA_BK, q0);
+          }
+        }
+      }
+      // Before shared memory is given up: every stage has been read by its MMAs (with CG == 2 the
+      // leader's commits arrive here too, so none may still be on its way), or, after an abort,
+      // every copy has landed.
+      const int64_t first = it > a.stages ? it - a.stages : 0;
+      for (int64_t j = first; j < it; ++j) {
+        int zero = 0;
+        uint64_t* bar = (ok && !*abort_flag) ? &ctl->empty[j % a.stages] : &ctl->full[j % a.stages];
+        if (CG == 2 && rank != 0 && (!ok || *abort_flag)) break;   // its copies signal the leader
+        if (!mbar_wait_bounded(bar, (uint32_t)((j / a.stages) & 1), &zero)) {
+          *abort_flag = 1;
+          atomicExch(a.status, KERR_DRAIN_TIMEOUT);
+          break;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer ------------------------------
+    if (lane == 0 && (CG == 1 || rank == 0)) {
+      const uint32_t fmt = a.bf16 ? 1u : 0u;
+      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.x_mn << 15) | ((uint32_t)a.y_mn << 16) |
+                             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+      const uint64_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
+      int64_t it = 0;
+      int local = 0;
+      bool ok = true;
+      for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+        const int buf = local & 1;
+        if (local >= 2 && !mbar_wait_bounded(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
+          if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
+          ok = false;
+          break;
+        }
+        ga_fence_after();
+        const uint32_t d = tmem_base + (uint32_t)(buf * BN);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = (int)(it % a.stages);
+          if (!mbar_wait_bounded(&ctl->full[s], (uint32_t)((it / a.stages) & 1), abort_flag)) {
+            if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_FULL_WAIT_TIMEOUT); }
+            ok = false;
+            break;
+          }
+          ga_fence_after();
+          const uint32_t x = smem_u32(smem) + s * a.stage_bytes;
+          const uint64_t dx = ga_desc(x, a.x_mn), dy = ga_desc(x + GA_X_BYTES, a.y_mn);
+#pragma unroll
+          for (int j = 0; j < GA_BK / 16; ++j)
+            ga_mma<CG>(d, dx + j * x_step, dy + j * y_step, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+          ga_commit<CG>(&ctl->empty[s]);
+        }
+        if (ok) ga_commit<CG>(&ctl->acc_full[buf]);
+      }
+    }
+  } else {
+    // ------------------------------ epilogue ------------------------------
+    const int quad = warp & 3, part = (warp - 2) >> 2;   // lanes of tensor memory; share of the columns
+    constexpr int W = BN >= 32 ? 32 : 16;
+    constexpr int PART_COLS = BN / (EW / 4);
+    int local = 0;
+    bool ok = true;
+    for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+      const int buf = local & 1;
+      const GaTile t = ga_tile(a, tile);
+      if (!mbar_wait_bounded(&ctl->acc_full[buf], (uint32_t)((local >> 1) & 1), abort_flag)) {
+        if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
+        ok = false;
+        break;
+      }
+      ga_fence_after();
+      const int64_t r = (int64_t)t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32 + lane;
+      const int64_t q = (int64_t)t.qt * BN + part * PART_COLS;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * PART_COLS);
+#pragma unroll 1
+      for (int c = 0; c < PART_COLS; c += W) {
+        float v[W];
+        ga_tmem_ld<W>(taddr + c, v);
+        if (a.kblocks == 0) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[j] = 0.0f;   // the accumulator was never written
+        }
+        if (split > 1) {
+          // column-major FP32 in the operand ring, which nothing reads any more
+          float* stage = reinterpret_cast<float*>(smem) + (part * PART_COLS + c) * 128 + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < W; ++j) stage[j * 128] = v[j];
+        } else {
+          ga_finish<QC, W>(a, r, q + c, v);
+        }
+      }
+      ga_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) arrive_cluster(map_rank(smem_u32(&ctl->acc_empty[buf]), 0));
+        else mbar_arrive(&ctl->acc_empty[buf]);
+      }
+    }
+  }
+
+  if (CG == 1 && split > 1) {
+    // ------------------------------ sum over the cluster ------------------------------
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2 && !*abort_flag) {
+      const int e = threadIdx.x - 64;                 // 0 .. EW * 32 - 1
+      const int row = e & 127, part = e >> 7;
+      const GaTile t = ga_tile(a, first_tile);
+      const int64_t r = (int64_t)t.rt * 128 + row;
+      const int cols = BN / split;                    // columns of this CTA
+      auto sum_run = [&](auto width) {
+        constexpr int W = decltype(width)::value;
+        for (int c = part * W; c < cols; c += W * (EW / 4)) {
+          const int col = (int)rank * cols + c;
+          float v[W];
+#pragma unroll
+          for (int j = 0; j < W; ++j) v[j] = 0.0f;
+          for (int s = 0; s < split; ++s) {
+            const uint32_t base = map_rank(smem_u32(smem) + (uint32_t)(col * 128 + row) * 4, s);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] += ld_cluster(base + j * 512);
+          }
+          ga_finish<QC, W>(a, r, (int64_t)t.qt * BN + col, v);
+        }
+      };
+      if (QC || cols >= 8) sum_run(ActC<8>());
+      else sum_run(ActC<2>());
+    }
+    __syncwarp();
+    cluster_sync();      // nobody leaves while its shared memory is still read
+  }
+
+  // ------------------------------ teardown ------------------------------
+  ga_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  if (warp == 1) {
+    if (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ copy to an aligned layout
+// Column `blockIdx.y`-th of a len x cols matrix at any 2-byte address and leading dimension to a
+// buffer whose columns start on 16-byte boundaries, so that TMA can read it. A thread makes one
+// aligned group of eight; in the middle of a column it takes the two aligned 16-byte words that
+// the group straddles and shifts them together, so both sides move at full width.
+__global__ void __launch_bounds__(256)
+align_copy_kernel(const uint16_t* __restrict__ src, int64_t ld_src, uint16_t* __restrict__ dst, int64_t ld_dst,
+                  int64_t len, int64_t cols) {
+  const int64_t groups = (len + 7) / 8;
+  const int64_t total = groups * cols;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t col = i / groups, g = i - col * groups;
+    const uint16_t* s = src + col * ld_src + g * 8;
+    uint4 o;
+    if (g > 0 && g + 2 < groups) {
+      const int shift = (int)(reinterpret_cast<uintptr_t>(s) & 15) * 8;   // bits
+      const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(s) & ~uintptr_t(15));
+      const uint4 lo = p[0], hi = p[1];   // inside the column: one group of eight lies on either side
+      const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      const int word = shift >> 5, bits = shift & 31;
+      uint32_t q[5];
+#pragma unroll
+      for (int j = 0; j < 5; ++j)
+        q[j] = word == 0 ? w[j] : word == 1 ? w[j + 1] : word == 2 ? w[j + 2] : w[j + 3 < 8 ? j + 3 : 7];
+      o.x = __funnelshift_r(q[0], q[1], bits);
+      o.y = __funnelshift_r(q[1], q[2], bits);
+      o.z = __funnelshift_r(q[2], q[3], bits);
+      o.w = __funnelshift_r(q[3], q[4], bits);
+    } else {
+      uint16_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = g * 8 + j < len ? s[j] : (uint16_t)0;
+      o.x = e[0] | (uint32_t)e[1] << 16;
+      o.y = e[2] | (uint32_t)e[3] << 16;
+      o.z = e[4] | (uint32_t)e[5] << 16;
+      o.w = e[6] | (uint32_t)e[7] << 16;
+    }
+    *reinterpret_cast<uint4*>(dst + col * ld_dst + g * 8) = o;
+  }
 }
 
 // ------------------------------------------------------------------ gradient of the epilogue
@@ -153,11 +655,184 @@ inline bool vec16(const void* p, int64_t ld) {
 
 }  // namespace
 
-cudaError_t launch_gemm_act(const GemmActProblem& p, cudaStream_t stream) {
-  if (p.M == 0 || p.N == 0) return cudaSuccess;
-  const dim3 grid((p.M + GA_TILE - 1) / GA_TILE, (p.N + GA_TILE - 1) / GA_TILE);
-  gemm_act_kernel<<<grid, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+// ------------------------------------------------------------------ choice of a variant
+namespace {
+
+// One way to run a product: orientation, tile, split of k.
+struct GaPlan {
+  bool qc;
+  int bn, cg, split;
+};
+
+constexpr int GA_SMS = 148;
+
+// Estimated clocks of a variant. Per 64-deep k block a CTA issues four MMAs of BN / 2 clocks each
+// and loads (128 + BN / CG) rows of 128 bytes at what an SM gets out of L2.
+double ga_cost(const GaPlan& v, int64_t M, int64_t N, int64_t K) {
+  const int64_t R = v.qc ? N : M, Q = v.qc ? M : N;
+  const int64_t tiles = ((R + 128 * v.cg - 1) / (128 * v.cg)) * ((Q + v.bn - 1) / v.bn);
+  const int64_t kb = (K + GA_BK - 1) / GA_BK;
+  const int64_t ctas = tiles * v.cg * v.split;
+  const double mma = 2.0 * std::max(v.bn, 32), load = (128.0 + (double)v.bn / v.cg) * 128.0 / 60.0;
+  const double per_kb = std::max(mma, load);
+  const int64_t waves = (ctas + GA_SMS - 1) / GA_SMS;
+  const int64_t run = (kb + v.split - 1) / v.split;
+  // the epilogue of a tile, of which only the last one is not under the MMAs of the next
+  const double epilogue = 128.0 * v.bn / 24.0 / v.split;
+  return waves * run * per_kb + epilogue + (v.split > 1 ? 1200.0 + 100.0 * v.split : 0.0) + 2000.0;
+}
+
+GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
+  GaPlan best{false, 16, 1, 1};
+  double best_cost = 1e300;
+  auto consider = [&](GaPlan v) {
+    const double c = ga_cost(v, M, N, K);
+    if (c < best_cost) {
+      best_cost = c;
+      best = v;
+    }
+  };
+  const int64_t kb = (K + GA_BK - 1) / GA_BK;
+  for (int qc = 0; qc < 2; ++qc) {
+    if (qc && !vec) continue;
+    for (int bn = qc ? 64 : 16; bn <= 256; bn *= 2) {
+      if (qc && bn == 256) consider({true, 256, 2, 1});
+      if (!qc && bn == 256) consider({false, 256, 2, 1});
+      if (bn <= 128)
+        for (int s = 1; s <= 8 && s <= std::max<int64_t>(kb, 1); s *= 2) consider({qc != 0, bn, 1, s});
+    }
+  }
+  return best;
+}
+
+template <int BN, int CG, bool QC>
+cudaError_t ga_launch(const CUtensorMap& mx, const CUtensorMap& my, GemmActKernelArgs& a, cudaStream_t stream) {
+  constexpr int YROWS = BN / CG;
+  const int y_bytes = (a.y_mn ? std::max(YROWS, 64) : YROWS) * 128;
+  a.stage_bytes = GA_X_BYTES + y_bytes;
+  const int budget = 200 * 1024;
+  a.stages = std::min(GA_MAX_STAGES, budget / a.stage_bytes);
+  int smem = a.stages * a.stage_bytes;
+  if (a.split > 1) smem = std::max(smem, BN * 128 * 4);
+  smem += 1024;
+  auto kernel = gemm_act_kernel<BN, CG, QC>;
+  static std::atomic<bool> configured[PARALIA_MAX_UNITS] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!configured[dev]) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)sizeof(GaCtl) - 1024);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  const int group = CG * a.split;
+  int64_t grid = a.tiles * group;
+  if (a.split == 1) grid = std::min<int64_t>(grid, GA_SMS / CG * CG);
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(GaShape<BN>::THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = group;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = group > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, mx, my, a);
+}
+
+// Whether TMA can read a stored operand of `cols` columns in place.
+bool ga_in_place(const void* p, int64_t ld, int64_t cols) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (cols <= 1 || (ld & 7) == 0);
+}
+
+}  // namespace
+
+int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0 || ga_in_place(p, ld, cols)) return 0;
+  return ((rows + 7) / 8 * 8 * cols * 2 + 255) / 256 * 256;
+}
+
+int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStream_t stream) {
+  if (p.M == 0 || p.N == 0) return PARALIA_OK;
+  const bool k_work = p.K > 0;
+  const void* A = p.A;
+  const void* B = p.B;
+  int64_t ldA = p.ldA, ldB = p.ldB;
+  const int64_t a_rows = p.ta ? p.K : p.M, a_cols = p.ta ? p.M : p.K;
+  const int64_t b_rows = p.tb ? p.N : p.K, b_cols = p.tb ? p.K : p.N;
+  if (k_work) {
+    char* s = static_cast<char*>(scratch);
+    auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) -> cudaError_t {
+      const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
+      const int64_t ld8 = (rows + 7) / 8 * 8;
+      if (bytes == 0) {
+        if (cols <= 1) ld = ld8;
+        return cudaSuccess;
+      }
+      const int64_t blocks = std::min<int64_t>((ld8 / 8 * cols + 255) / 256, GA_SMS * 16);
+      align_copy_kernel<<<(int)blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(q), ld,
+                                                         reinterpret_cast<uint16_t*>(s), ld8, rows, cols);
+      q = s;
+      ld = ld8;
+      s += bytes;
+      return cudaGetLastError();
+    };
+    PL_CUDA(in_reach(A, ldA, a_rows, a_cols));
+    PL_CUDA(in_reach(B, ldB, b_rows, b_cols));
+  }
+  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
+  const bool vec = vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) &&
+                   vec16(p.bias, 0);
+  GaPlan v = ga_choose(p.M, p.N, p.K, vec);
+
+  GemmActKernelArgs a;
+  memset(&a, 0, sizeof(a));
+  a.bias = p.bias; a.C = p.C; a.D = p.D; a.pre = p.pre;
+  a.ldC = p.ldC; a.ldD = p.ldD; a.ldPre = p.ldPre;
+  a.M = p.M; a.N = p.N;
+  a.act = p.act; a.bf16 = p.bf16; a.alpha = p.alpha; a.beta = p.beta;
+  a.vec = vec;
+  a.status = status;
+  a.kblocks = (p.K + GA_BK - 1) / GA_BK;
+  a.split = v.split;
+  const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
+  const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
+  a.tiles = r_tiles * q_tiles;
+  a.r_tiles = (int32_t)r_tiles;
+  a.q_tiles = (int32_t)q_tiles;
+  // op(A) is stored with k contiguous if it is a transpose, op(B) if it is not
+  const bool a_k = p.ta != 0, b_k = p.tb == 0;
+  a.x_mn = v.qc ? !b_k : !a_k;
+  a.y_mn = v.qc ? !a_k : !b_k;
+  CUtensorMap mx, my;
+  memset(&mx, 0, sizeof(mx));
+  memset(&my, 0, sizeof(my));
+  if (k_work) {
+    const int yrows = v.bn / v.cg;
+    PL_TRY(make_tensor_map(v.qc ? &my : &mx, A, 2, a_rows, a_cols, 1, ldA * 2, (uint64_t)ldA * a_cols * 2, 64,
+                           a_k ? (v.qc ? yrows : 128) : 64));
+    PL_TRY(make_tensor_map(v.qc ? &mx : &my, B, 2, b_rows, b_cols, 1, ldB * 2, (uint64_t)ldB * b_cols * 2, 64,
+                           b_k ? (v.qc ? 128 : yrows) : 64));
+  }
+  cudaError_t e = cudaErrorInvalidValue;
+#define GA_CASE(BN, CG, QC) \
+  if (v.bn == BN && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(mx, my, a, stream);
+  GA_CASE(16, 1, false)
+  GA_CASE(32, 1, false)
+  GA_CASE(64, 1, false)
+  GA_CASE(128, 1, false)
+  GA_CASE(256, 2, false)
+  GA_CASE(64, 1, true)
+  GA_CASE(128, 1, true)
+  GA_CASE(256, 2, true)
+#undef GA_CASE
+  PL_CUDA(e);
+  return PARALIA_OK;
 }
 
 int act_grad_chunks(int64_t M, int64_t N) {

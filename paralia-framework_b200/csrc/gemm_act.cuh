@@ -24,7 +24,12 @@ struct GemmActProblem {
   float alpha, beta;
 };
 
-cudaError_t launch_gemm_act(const GemmActProblem& p, cudaStream_t stream);
+// Bytes of the aligned copy that a stored rows x cols operand needs before TMA can read it; 0 if it
+// is read in place. A multiple of 256.
+int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols);
+// `scratch` (16-byte aligned) holds the copies of A and of B; `status` is the GPU's word for waits
+// that gave up. Returns a PARALIA_* code.
+int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStream_t stream);
 
 // dZ <- dD * act'(pre) (dZ may be null; pre is not read for PARALIA_ACT_NONE), and, where
 // dbias is not null, dbias <- row sums of the unrounded product + beta_bias * dbias.

@@ -36,14 +36,26 @@ int check_common(int type, char TransA, char TransB, int64_t M, int64_t N, int64
   return PARALIA_OK;
 }
 
+int check_scratch(const void* scratch, int64_t have, int64_t need) {
+  if (!scratch || have < need)
+    return fail(PARALIA_ERR_INVALID_ARG, "the call needs %lld bytes of scratch, %lld were given", (long long)need,
+                (long long)(scratch ? have : 0));
+  if (reinterpret_cast<uintptr_t>(scratch) & 15)
+    return fail(PARALIA_ERR_INVALID_ARG, "scratch is not aligned to 16 bytes");
+  return PARALIA_OK;
+}
+
 bool odd_address(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
 
 }  // namespace
 
 int64_t gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
                                const void* A, int64_t ldA, const void* B, int64_t ldB) {
-  (void)type; (void)TransA; (void)TransB; (void)M; (void)N; (void)K; (void)A; (void)ldA; (void)B; (void)ldB;
-  return 0;
+  if (check_common(type, TransA, TransB, M, N, K, 1.0f, ldA, ldB, PARALIA_ACT_NONE) != PARALIA_OK) return 0;
+  if (M == 0 || N == 0 || K == 0) return 0;
+  const bool ta = is_trans(TransA), tb = is_trans(TransB);
+  return gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K) +
+         gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N);
 }
 
 int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
@@ -63,6 +75,8 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   if (D == A || D == B || D == pre || D == bias || (pre && (pre == A || pre == B || pre == bias)) ||
       (beta != 0.0f && (pre == C || (D == C && ldD != ldC))))
     return fail(PARALIA_ERR_INVALID_ARG, "an output may share memory with no operand, but D with C at the same leading dimension");
+  const int64_t need = product ? gemm_act_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB) : 0;
+  if (need > 0) PL_TRY(check_scratch(scratch, scratch_bytes, need));
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -76,24 +90,27 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   p.ta = is_trans(TransA); p.tb = is_trans(TransB);
   p.act = act; p.bf16 = type == PARALIA_BF16;
   p.alpha = alpha; p.beta = beta;
-  (void)scratch; (void)scratch_bytes;
-  PL_CUDA(launch_gemm_act(p, static_cast<cudaStream_t>(stream)));
-  return PARALIA_OK;
+  return launch_gemm_act(p, scratch, rt.dev(dev).status_dev, static_cast<cudaStream_t>(stream));
 }
 
 namespace {
 
-// Scratch of the gradient: dZ (M x N, leading dimension a multiple of eight), then the
-// partial row sums of the bias gradient.
+// Scratch of the gradient: dZ (M x N, leading dimension a multiple of eight; without an
+// activation the aligned copy of dD where it needs one), then the partial row sums of the bias
+// gradient, then the aligned copies of A and of B where they need one. Only one product runs at
+// a time and each takes one of the two operands, so the copies share their place.
 struct GradScratch {
-  int64_t ldZ, z_bytes, partial_bytes, total;
+  int64_t ldZ, z_bytes, partial_bytes, copy_bytes, total;
 };
-GradScratch grad_scratch(int64_t M, int64_t N) {
+GradScratch grad_scratch(int64_t M, int64_t N, int64_t K, bool ta, bool tb, const void* A, int64_t ldA, const void* B,
+                         int64_t ldB) {
   GradScratch g;
   g.ldZ = round_up(std::max<int64_t>(1, M), 8);
   g.z_bytes = round_up(g.ldZ * N * 2, 256);
   g.partial_bytes = round_up((int64_t)act_grad_chunks(M, N) * M * (int64_t)sizeof(float), 256);
-  g.total = g.z_bytes + g.partial_bytes;
+  g.copy_bytes = std::max(gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K),
+                          gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N));
+  g.total = g.z_bytes + g.partial_bytes + g.copy_bytes;
   return g;
 }
 
@@ -101,9 +118,8 @@ GradScratch grad_scratch(int64_t M, int64_t N) {
 
 int64_t gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
                                     const void* A, int64_t ldA, const void* B, int64_t ldB, int act) {
-  (void)A; (void)B;
   if (check_common(type, TransA, TransB, M, N, K, 1.0f, ldA, ldB, act) != PARALIA_OK) return 0;
-  return grad_scratch(M, N).total;
+  return grad_scratch(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB).total;
 }
 
 int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
@@ -134,12 +150,8 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
     if (outs[i] == A || outs[i] == B || outs[i] == pre || outs[i] == dD || outs[i] == outs[(i + 1) % 3])
       return fail(PARALIA_ERR_INVALID_ARG, "a gradient may share memory with no operand and no other gradient");
   }
-  const GradScratch g = grad_scratch(M, N);
-  if (!scratch || scratch_bytes < g.total)
-    return fail(PARALIA_ERR_INVALID_ARG, "the gradient needs %lld bytes of scratch, %lld were given",
-                (long long)g.total, (long long)(scratch ? scratch_bytes : 0));
-  if (reinterpret_cast<uintptr_t>(scratch) & 15)
-    return fail(PARALIA_ERR_INVALID_ARG, "scratch is not aligned to 16 bytes");
+  const GradScratch g = grad_scratch(M, N, K, ta, tb, A, ldA, B, ldB);
+  PL_TRY(check_scratch(scratch, scratch_bytes, g.total));
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -148,8 +160,10 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = type == PARALIA_BF16;
 
-  // dZ and the bias gradient in one pass over dD and pre. Without an activation dZ is dD.
-  const bool need_z = entries && uses_pre && (want_a || want_b);
+  // dZ and the bias gradient in one pass over dD and pre. Without an activation dZ is dD, in
+  // place if TMA can read it there.
+  const bool products = entries && K > 0 && alpha != 0.0f && (want_a || want_b);
+  const bool need_z = products && (uses_pre || gemm_act_operand_copy_bytes(dD, lddD, M, N) > 0);
   char* base = static_cast<char*>(scratch);
   if (need_z || want_bias) {
     ActGradProblem a;
@@ -162,6 +176,8 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   }
   const void* dZ = need_z ? base : dD;
   const int64_t ldZ = need_z ? g.ldZ : lddD;
+  void* copies = base + g.z_bytes + g.partial_bytes;
+  int* status = rt.dev(dev).status_dev;
 
   GemmActProblem p;
   memset(&p, 0, sizeof(p));
@@ -179,7 +195,7 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
       p.A = dZ; p.ldA = ldZ; p.ta = 1; p.B = A; p.ldB = ldA; p.tb = ta;
       p.M = (int32_t)N; p.N = (int32_t)K;
     }
-    PL_CUDA(launch_gemm_act(p, s));
+    PL_TRY(launch_gemm_act(p, copies, status, s));
   }
   if (want_a) {
     // d op(A) = alpha dZ op(B)^T, stored as A is
@@ -192,7 +208,7 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
       p.A = B; p.ldA = ldB; p.ta = tb; p.B = dZ; p.ldB = ldZ; p.tb = 1;
       p.M = (int32_t)K; p.N = (int32_t)M;
     }
-    PL_CUDA(launch_gemm_act(p, s));
+    PL_TRY(launch_gemm_act(p, copies, status, s));
   }
   return PARALIA_OK;
 }

@@ -155,8 +155,9 @@ def test_infinities_and_nans_stay_where_they_are(pl):
         A.t[0, 9] = float("-inf")
         for act, low in (("none", float("-inf")), ("relu", 0.0), ("gelu", 0.0), ("gelu_tanh", 0.0), ("silu", 0.0)):
             D = d.Mat(M, N, torch.bfloat16)
+            n = pl.tile_gemm_act_scratch_bytes(pl.BF16, "T", "N", M, N, K, A.addr, A.ld, B.addr, B.ld)
             pl.tile_gemm_act(0, pl.BF16, "T", "N", M, N, K, 1.0, A.addr, A.ld, B.addr, B.ld, 0.0, None, 1, D.addr, D.ld,
-                             act=d.ACTS.index(act))
+                             act=d.ACTS.index(act), scratch=_scratch(n), scratch_bytes=n)
             torch.cuda.synchronize()
             assert bool(torch.isposinf(D.t[7]).all()), act
             assert bool(torch.isnan(D.t[150]).all()), act
