@@ -353,16 +353,15 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (warp == 0) {
     // ------------------------------ producer ------------------------------
     if (lane == 0) {
-      int64_t it = 0;
+      int s = 0, filled = 0;         // stage, and how many stages have been filled at all (capped)
+      uint32_t phase = 0;            // parity of the ring's round
       bool ok = true;
       for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
         const GaTile t = ga_tile(a, tile);
         const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
         const int q0 = t.qt * BN + (CG == 2 ? (int)rank * YROWS : 0);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = (int)(it % a.stages);
-          const int64_t use = it / a.stages;
-          if (use > 0 && !mbar_wait_bounded(&ctl->empty[s], (uint32_t)((use - 1) & 1), abort_flag)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (filled == a.stages && !mbar_wait_bounded(&ctl->empty[s], phase ^ 1u, abort_flag)) {
             if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_EMPTY_WAIT_TIMEOUT); }
             ok = false;
             break;
@@ -383,17 +382,21 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           } else {
             ga_load<CG>(y, &map_y, bar, kb * GA_BK, q0);
           }
+          if (filled < a.stages) ++filled;
+          if (++s == a.stages) { s = 0; phase ^= 1u; }
         }
       }
       // Before shared memory is given up: every stage has been read by its MMAs (with CG == 2 the
       // leader's commits arrive here too, so none may still be on its way), or, after an abort,
       // every copy has landed.
-      const int64_t first = it > a.stages ? it - a.stages : 0;
-      for (int64_t j = first; j < it; ++j) {
+      for (int j = 0; j < filled; ++j) {
+        // the oldest stage first; `s` and `phase` are those of the next fill
         int zero = 0;
-        uint64_t* bar = (ok && !*abort_flag) ? &ctl->empty[j % a.stages] : &ctl->full[j % a.stages];
+        const int q = filled < a.stages ? j : (s + j < a.stages ? s + j : s + j - a.stages);
+        const uint32_t parity = filled < a.stages || q < s ? phase : phase ^ 1u;
+        uint64_t* bar = (ok && !*abort_flag) ? &ctl->empty[q] : &ctl->full[q];
         if (CG == 2 && rank != 0 && (!ok || *abort_flag)) break;   // its copies signal the leader
-        if (!mbar_wait_bounded(bar, (uint32_t)((j / a.stages) & 1), &zero)) {
+        if (!mbar_wait_bounded(bar, parity, &zero)) {
           *abort_flag = 1;
           atomicExch(a.status, KERR_DRAIN_TIMEOUT);
           break;
@@ -407,7 +410,8 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.x_mn << 15) | ((uint32_t)a.y_mn << 16) |
                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
       const uint64_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
-      int64_t it = 0;
+      int s = 0;
+      uint32_t phase = 0;
       int local = 0;
       bool ok = true;
       for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
@@ -419,9 +423,8 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         ga_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(buf * BN);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = (int)(it % a.stages);
-          if (!mbar_wait_bounded(&ctl->full[s], (uint32_t)((it / a.stages) & 1), abort_flag)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_bounded(&ctl->full[s], phase, abort_flag)) {
             if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_FULL_WAIT_TIMEOUT); }
             ok = false;
             break;
@@ -433,6 +436,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           for (int j = 0; j < GA_BK / 16; ++j)
             ga_mma<CG>(d, dx + j * x_step, dy + j * y_step, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
           ga_commit<CG>(&ctl->empty[s]);
+          if (++s == a.stages) { s = 0; phase ^= 1u; }
         }
         if (ok) ga_commit<CG>(&ctl->acc_full[buf]);
       }
