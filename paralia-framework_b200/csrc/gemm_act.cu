@@ -49,7 +49,13 @@ namespace {
 constexpr int GA_BK = 64;              // k per stage: 128 bytes, one swizzle row
 constexpr int GA_MAX_STAGES = 12;
 constexpr int GA_X_BYTES = 128 * GA_BK * 2;
+constexpr int GA_SMEM = 224 * 1024;    // operand ring and staging buffers
 constexpr int GA_PANEL = 8;            // q tiles per panel of the tile numbering
+
+// How an operand lies in memory and comes: k contiguous; r / q contiguous, one box for 64 of
+// them; r / q contiguous and a multiple of 64 of them, one box for all of a tile (the tensor map
+// then has the blocks of 64 as a dimension of its own).
+enum : int { GA_K_MAJOR = 0, GA_MN_BOXES = 1, GA_MN_BLOCKS = 2 };
 
 struct GemmActKernelArgs {
   const void* bias;
@@ -63,9 +69,10 @@ struct GemmActKernelArgs {
   int32_t kblocks;
   int32_t stages, stage_bytes;   // per CTA
   int32_t split;                 // CTAs that share a tile's k (the cluster, CG == 1)
-  int32_t x_mn, y_mn;            // 1: r / q contiguous, 0: k contiguous
+  int32_t x_mn, y_mn;            // GA_K_MAJOR, GA_MN_BOXES or GA_MN_BLOCKS
   int32_t act, bf16;
   int32_t vec;                   // D, C, pre and bias allow 16-byte accesses along M
+  int32_t stage_out;             // results leave through shared memory by TMA (QC, no split)
   float alpha, beta;
   int* status;
 };
@@ -112,18 +119,18 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 // Tiled TMA load without multicast; `bar` is a shared::cluster address. With CG == 2 it may lie in
 // the other CTA of the pair.
 template <int CG>
-__device__ __forceinline__ void ga_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+__device__ __forceinline__ void ga_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2 = 0) {
   if (CG == 2)
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
         "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
-        "r"(c1), "r"(0)
+        "r"(c1), "r"(c2)
         : "memory");
   else
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
         "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
-        "r"(c1), "r"(0)
+        "r"(c1), "r"(c2)
         : "memory");
 }
 
@@ -169,6 +176,21 @@ __device__ __forceinline__ void ga_commit(uint64_t* bar) {
                  : "memory");
 }
 
+// TMA store of a 64-column x 32-row box from shared memory, and the waits for it.
+__device__ __forceinline__ void ga_store(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(src), "r"(c0), "r"(c1), "r"(0)
+               : "memory");
+}
+__device__ __forceinline__ void ga_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void ga_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void ga_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
+
 __device__ __forceinline__ void ga_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ga_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -207,28 +229,50 @@ __device__ __forceinline__ void ga_tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
 }
 
 // ------------------------------------------------------------------ epilogue
-// Eight neighbouring rows m .. m+7 of column n of D (QC): acc -> D, pre.
+// Eight neighbouring rows of one column of D: from sums, bias and C to packed D and Z.
+template <int ACT>
+__device__ __forceinline__ void ga_eval8(const GemmActKernelArgs& a, const float* v, const uint4& b, const uint4& c,
+                                         uint32_t (&d)[4], uint32_t (&z)[4]) {
+  const bool bf = a.bf16 != 0;
+  const uint32_t cv[4] = {c.x, c.y, c.z, c.w}, bv[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 bb = unpack16(bv[i], bf), cc = unpack16(cv[i], bf);
+    const float z0 = fmaf(a.alpha, v[2 * i], bb.x), z1 = fmaf(a.alpha, v[2 * i + 1], bb.y);
+    z[i] = pack16(z0, z1, bf);
+    float d0 = act_value<ACT>(z0), d1 = act_value<ACT>(z1);
+    if (a.C) {
+      d0 = fmaf(a.beta, cc.x, d0);
+      d1 = fmaf(a.beta, cc.y, d1);
+    }
+    d[i] = pack16(d0, d1, bf);
+  }
+}
+// Eight 16-bit elements of which `valid` exist; the others are 0 and not read.
+__device__ __forceinline__ uint4 ga_load8(const void* p, int64_t valid) {
+  if (valid >= 8) return *static_cast<const uint4*>(p);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < valid) w[i >> 1] |= (uint32_t)static_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 ga_load_bias8(const GemmActKernelArgs& a, int64_t m) {
+  if (!a.bias) return make_uint4(0, 0, 0, 0);
+  return ga_load8(static_cast<const uint16_t*>(a.bias) + m, a.M - m);
+}
+__device__ __forceinline__ uint4 ga_load_c8(const GemmActKernelArgs& a, int64_t m, int64_t n) {
+  if (!a.C) return make_uint4(0, 0, 0, 0);
+  return ga_load8(static_cast<const uint16_t*>(a.C) + m + n * a.ldC, a.M - m);
+}
+
+// Rows m .. m+7 of column n of D (QC): acc -> D, pre.
 template <int ACT>
 __device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m, int64_t n, float* v) {
   const bool bf = a.bf16 != 0;
   if (a.vec && m + 8 <= a.M) {
-    uint4 c = make_uint4(0, 0, 0, 0), b = make_uint4(0, 0, 0, 0);
-    if (a.C) c = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.C) + m + n * a.ldC);
-    if (a.bias) b = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.bias) + m));
-    const uint32_t cv[4] = {c.x, c.y, c.z, c.w}, bv[4] = {b.x, b.y, b.z, b.w};
     uint32_t z[4], d[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 bb = unpack16(bv[i], bf), cc = unpack16(cv[i], bf);
-      const float z0 = fmaf(a.alpha, v[2 * i], bb.x), z1 = fmaf(a.alpha, v[2 * i + 1], bb.y);
-      z[i] = pack16(z0, z1, bf);
-      float d0 = act_value<ACT>(z0), d1 = act_value<ACT>(z1);
-      if (a.C) {
-        d0 = fmaf(a.beta, cc.x, d0);
-        d1 = fmaf(a.beta, cc.y, d1);
-      }
-      d[i] = pack16(d0, d1, bf);
-    }
+    ga_eval8<ACT>(a, v, ga_load_bias8(a, m), ga_load_c8(a, m, n), d, z);
     if (a.pre) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.pre) + m + n * a.ldPre) = make_uint4(z[0], z[1], z[2], z[3]);
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.D) + m + n * a.ldD) = make_uint4(d[0], d[1], d[2], d[3]);
     return;
@@ -296,6 +340,7 @@ __device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int64_t ti
 template <int BN, int CG, bool QC>
 __global__ void __launch_bounds__(GaShape<BN>::THREADS, 1)
 gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_pre,
                 const __grid_constant__ GemmActKernelArgs a) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
@@ -370,13 +415,17 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           uint32_t bar = smem_u32(&ctl->full[s]);
           if (CG == 2) bar = map_rank(bar, 0);
           if (CG == 1 || rank == 0) mbar_expect_tx(&ctl->full[s], a.stage_bytes * CG);
-          if (a.x_mn) {
+          if (a.x_mn == GA_MN_BLOCKS) {
+            ga_load<CG>(x, &map_x, bar, 0, kb * GA_BK, r0 / 64);
+          } else if (a.x_mn) {
             ga_load<CG>(x, &map_x, bar, r0, kb * GA_BK);
             ga_load<CG>(x + 8192, &map_x, bar, r0 + 64, kb * GA_BK);
           } else {
             ga_load<CG>(x, &map_x, bar, kb * GA_BK, r0);
           }
-          if (a.y_mn) {
+          if (YROWS >= 64 && a.y_mn == GA_MN_BLOCKS) {
+            ga_load<CG>(y, &map_y, bar, 0, kb * GA_BK, q0 / 64);
+          } else if (a.y_mn) {
 #pragma unroll
             for (int j = 0; j < (YROWS + 63) / 64; ++j) ga_load<CG>(y + j * 8192, &map_y, bar, q0 + j * 64, kb * GA_BK);
           } else {
@@ -407,7 +456,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // ------------------------------ MMA issuer ------------------------------
     if (lane == 0 && (CG == 1 || rank == 0)) {
       const uint32_t fmt = a.bf16 ? 1u : 0u;
-      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.x_mn << 15) | ((uint32_t)a.y_mn << 16) |
+      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a.x_mn ? 1u << 15 : 0u) | (a.y_mn ? 1u << 16 : 0u) |
                              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
       const uint64_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
       int s = 0;
@@ -444,7 +493,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else {
     // ------------------------------ epilogue ------------------------------
     const int quad = warp & 3, part = (warp - 2) >> 2;   // lanes of tensor memory; share of the columns
-    constexpr int W = BN >= 32 ? 32 : 16;
+    constexpr int W = QC && BN >= 32 ? 32 : 16;
     constexpr int PART_COLS = BN / (EW / 4);
     int local = 0;
     bool ok = true;
@@ -460,8 +509,56 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const int64_t r = (int64_t)t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32 + lane;
       const int64_t q = (int64_t)t.qt * BN + part * PART_COLS;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * PART_COLS);
+      if constexpr (QC) {
+        if (a.stage_out) {
+          // 64 columns x 32 rows at a time through this warp's staging buffers (128-byte rows,
+          // swizzled as the tensor map says), written out by TMA: whole lines leave, edges are
+          // clipped by the map, and the store runs under the next columns' arithmetic
+          const uint32_t out = smem_u32(smem) + a.stages * a.stage_bytes + (warp - 2) * (a.pre ? 8192 : 4096);
+          const uint32_t row = out + lane * 128;
+          const int r_first = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32;
+          const bool row_in = r < a.N;
 #pragma unroll 1
-      for (int c = 0; c < PART_COLS; c += W) {
+          for (int c = 0; c < PART_COLS; c += 64) {
+            if (q + c >= a.M) break;
+            if (lane == 0) ga_store_wait_read();
+            __syncwarp();
+#pragma unroll 1
+            for (int h = 0; h < 64; h += 32) {
+              uint4 cc[4];
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                cc[g] = row_in ? ga_load_c8(a, q + c + h + 8 * g, r) : make_uint4(0, 0, 0, 0);
+              float v[32];
+              ga_tmem_ld<32>(taddr + c + h, v);
+              if (a.kblocks == 0) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+              }
+              with_act(a.act, [&](auto k) {
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  const int64_t m = q + c + h + 8 * g;
+                  uint32_t d[4], z[4];
+                  ga_eval8<decltype(k)::value>(a, &v[8 * g], ga_load_bias8(a, m), cc[g], d, z);
+                  const uint32_t at = row + (((h >> 3) + g) ^ (lane & 7)) * 16;
+                  st_shared16(at, d);
+                  if (a.pre) st_shared16(at + 4096, z);
+                }
+              });
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && r_first < a.N) {
+              ga_store(&map_d, out, (int)(q + c), r_first);
+              if (a.pre) ga_store(&map_pre, out + 4096, (int)(q + c), r_first);
+              ga_store_commit();
+            }
+          }
+        }
+      }
+#pragma unroll 1
+      for (int c = 0; c < PART_COLS && !(QC && a.stage_out); c += W) {
         float v[W];
         ga_tmem_ld<W>(taddr + c, v);
         if (a.kblocks == 0) {
@@ -484,6 +581,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         else mbar_arrive(&ctl->acc_empty[buf]);
       }
     }
+    if (QC && lane == 0) ga_store_wait();
   }
 
   if (CG == 1 && split > 1) {
@@ -697,10 +795,9 @@ GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
     }
   };
   const int64_t kb = (K + GA_BK - 1) / GA_BK;
-  for (int qc = 0; qc < 2; ++qc) {
-    if (qc && !vec) continue;
+  for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
     for (int bn = qc ? 64 : 16; bn <= 256; bn *= 2) {
-      if (qc && bn == 256) consider({true, 256, 2, 1});
+      if (qc && bn >= 128) consider({true, bn, 2, 1});
       if (!qc && bn == 256) consider({false, 256, 2, 1});
       if (bn <= 128)
         for (int s = 1; s <= 8 && s <= std::max<int64_t>(kb, 1); s *= 2) consider({qc != 0, bn, 1, s});
@@ -710,13 +807,13 @@ GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
 }
 
 template <int BN, int CG, bool QC>
-cudaError_t ga_launch(const CUtensorMap& mx, const CUtensorMap& my, GemmActKernelArgs& a, cudaStream_t stream) {
+cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaStream_t stream) {
   constexpr int YROWS = BN / CG;
   const int y_bytes = (a.y_mn ? std::max(YROWS, 64) : YROWS) * 128;
   a.stage_bytes = GA_X_BYTES + y_bytes;
-  const int budget = 200 * 1024;
-  a.stages = std::min(GA_MAX_STAGES, budget / a.stage_bytes);
-  int smem = a.stages * a.stage_bytes;
+  const int staging = a.stage_out ? GaShape<BN>::EPILOGUE_WARPS * (a.pre ? 8192 : 4096) : 0;
+  a.stages = std::min(GA_MAX_STAGES, (GA_SMEM - staging) / a.stage_bytes);
+  int smem = a.stages * a.stage_bytes + staging;
   if (a.split > 1) smem = std::max(smem, BN * 128 * 4);
   smem += 1024;
   auto kernel = gemm_act_kernel<BN, CG, QC>;
@@ -725,7 +822,7 @@ cudaError_t ga_launch(const CUtensorMap& mx, const CUtensorMap& my, GemmActKerne
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (!configured[dev]) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)sizeof(GaCtl) - 1024);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GA_SMEM + 1024);
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
@@ -746,7 +843,7 @@ cudaError_t ga_launch(const CUtensorMap& mx, const CUtensorMap& my, GemmActKerne
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = group > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, mx, my, a);
+  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a);
 }
 
 // Whether TMA can read a stored operand of `cols` columns in place.
@@ -811,21 +908,28 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   a.q_tiles = (int32_t)q_tiles;
   // op(A) is stored with k contiguous if it is a transpose, op(B) if it is not
   const bool a_k = p.ta != 0, b_k = p.tb == 0;
-  a.x_mn = v.qc ? !b_k : !a_k;
-  a.y_mn = v.qc ? !a_k : !b_k;
-  CUtensorMap mx, my;
-  memset(&mx, 0, sizeof(mx));
-  memset(&my, 0, sizeof(my));
-  if (k_work) {
-    const int yrows = v.bn / v.cg;
-    PL_TRY(make_tensor_map(v.qc ? &my : &mx, A, 2, a_rows, a_cols, 1, ldA * 2, (uint64_t)ldA * a_cols * 2, 64,
-                           a_k ? (v.qc ? yrows : 128) : 64));
-    PL_TRY(make_tensor_map(v.qc ? &mx : &my, B, 2, b_rows, b_cols, 1, ldB * 2, (uint64_t)ldB * b_cols * 2, 64,
-                           b_k ? (v.qc ? 128 : yrows) : 64));
+  const int yrows = v.bn / v.cg, xrows = 128;
+  CUtensorMap maps[4];   // X, Y, D, pre
+  memset(maps, 0, sizeof(maps));
+  // `inner` x `outer` as stored; `k_major`: inner is k
+  auto operand = [&](CUtensorMap* map, const void* q, int64_t ld, int64_t inner, int64_t outer, bool k_major, int rows,
+                     int32_t* how) -> int {
+    *how = k_major ? GA_K_MAJOR : inner % 64 == 0 && rows >= 64 ? GA_MN_BLOCKS : GA_MN_BOXES;
+    if (!k_work) return PARALIA_OK;
+    if (*how == GA_MN_BLOCKS)
+      return make_tensor_map(map, q, 2, 64, outer, inner / 64, ld * 2, 128, 64, 64, rows / 64);
+    return make_tensor_map(map, q, 2, inner, outer, 1, ld * 2, (uint64_t)ld * outer * 2, 64, k_major ? rows : 64);
+  };
+  PL_TRY(operand(&maps[v.qc ? 1 : 0], A, ldA, a_rows, a_cols, a_k, v.qc ? yrows : xrows, v.qc ? &a.y_mn : &a.x_mn));
+  PL_TRY(operand(&maps[v.qc ? 0 : 1], B, ldB, b_rows, b_cols, b_k, v.qc ? xrows : yrows, v.qc ? &a.x_mn : &a.y_mn));
+  a.stage_out = v.qc && v.split == 1;
+  if (a.stage_out) {
+    PL_TRY(make_tensor_map(&maps[2], p.D, 2, p.M, p.N, 1, p.ldD * 2, (uint64_t)p.ldD * p.N * 2, 64, 32));
+    if (p.pre) PL_TRY(make_tensor_map(&maps[3], p.pre, 2, p.M, p.N, 1, p.ldPre * 2, (uint64_t)p.ldPre * p.N * 2, 64, 32));
   }
   cudaError_t e = cudaErrorInvalidValue;
 #define GA_CASE(BN, CG, QC) \
-  if (v.bn == BN && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(mx, my, a, stream);
+  if (v.bn == BN && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, a, stream);
   GA_CASE(16, 1, false)
   GA_CASE(32, 1, false)
   GA_CASE(64, 1, false)
@@ -833,6 +937,7 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   GA_CASE(256, 2, false)
   GA_CASE(64, 1, true)
   GA_CASE(128, 1, true)
+  GA_CASE(128, 2, true)
   GA_CASE(256, 2, true)
 #undef GA_CASE
   PL_CUDA(e);

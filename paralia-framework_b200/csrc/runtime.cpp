@@ -430,12 +430,12 @@ static EncodeTiledFn encode_tiled_fn() {
 
 int make_tensor_map(CUtensorMap* map, const void* base, int esz, uint64_t d0, uint64_t d1,
                     uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
-                    uint32_t box1) {
+                    uint32_t box1, uint32_t box2) {
   EncodeTiledFn fn = encode_tiled_fn();
   if (!fn) return fail(PARALIA_ERR_CUDA, "driver entry point cuTensorMapEncodeTiled not found");
   const cuuint64_t dims[3] = {d0, d1, d2};
   const cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
-  const cuuint32_t box[3] = {box0, box1, 1};
+  const cuuint32_t box[3] = {box0, box1, box2};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUtensorMapDataType dt = esz == 8   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT64
                                  : esz == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32

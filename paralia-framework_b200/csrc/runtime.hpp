@@ -154,7 +154,7 @@ int resolve_operand_location(const void* ptr, int loc_in, size_t bytes, int ngpu
 // 128-byte swizzle and zero fill outside the tensor.
 int make_tensor_map(CUtensorMap* map, const void* base, int esz, uint64_t d0, uint64_t d1,
                     uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t box0,
-                    uint32_t box1);
+                    uint32_t box1, uint32_t box2 = 1);
 
 // True if TMA can address a matrix at `base` with leading dimension ld (elements of esz bytes).
 inline bool tma_addressable(const void* base, int64_t ld, int esz) {
