@@ -36,6 +36,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstring>
+#include <utility>
 
 #include "act_math.cuh"
 #include "runtime.hpp"
@@ -50,7 +51,6 @@ constexpr int GA_BK = 64;              // k per stage: 128 bytes, one swizzle ro
 constexpr int GA_MAX_STAGES = 12;
 constexpr int GA_X_BYTES = 128 * GA_BK * 2;
 constexpr int GA_SMEM = 224 * 1024;    // operand ring and staging buffers
-constexpr int GA_PANEL = 8;            // q tiles per panel of the tile numbering
 
 // How an operand lies in memory and comes: k contiguous; r / q contiguous, one box for 64 of
 // them; r / q contiguous and a multiple of 64 of them, one box for all of a tile (the tensor map
@@ -66,7 +66,9 @@ struct GemmActKernelArgs {
   int64_t tiles;
   int32_t M, N;
   int32_t r_tiles, q_tiles;
+  int32_t panel;                 // q tiles per panel of the tile numbering
   int32_t kblocks;
+  int32_t bn;                    // columns of a tile: BN, or for BN = 64 any multiple of 16 up to it
   int32_t stages, stage_bytes;   // per CTA
   int32_t split;                 // CTAs that share a tile's k (the cluster, CG == 1)
   int32_t x_mn, y_mn;            // GA_K_MAJOR, GA_MN_BOXES or GA_MN_BLOCKS
@@ -103,6 +105,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// Programmatic dependent launch: wait until the kernels this one depends on have completed and
+// their writes are visible; allow the next kernel to be set up on free resources.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   uint32_t r;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
@@ -116,21 +122,42 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr) {
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// L2 keeps a line of the streamed operand no longer than it has to: it is read by the CTAs of one
+// round of tiles at about the same time, while the panel of the other operand comes again.
+__device__ __forceinline__ uint64_t ga_policy_stream() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t ga_policy_normal() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// A bounded wait by a whole warp, with one outcome.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag));
+}
 // Tiled TMA load without multicast; `bar` is a shared::cluster address. With CG == 2 it may lie in
 // the other CTA of the pair.
 template <int CG>
-__device__ __forceinline__ void ga_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2 = 0) {
+__device__ __forceinline__ void ga_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, uint64_t policy, int c0, int c1, int c2 = 0) {
   if (CG == 2)
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
-        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
-        "r"(c1), "r"(c2)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint "
+        "[%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "l"(policy)
         : "memory");
   else
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
-        "r"(c1), "r"(c2)
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0),
+        "r"(c1), "r"(c2), "l"(policy)
         : "memory");
 }
 
@@ -249,13 +276,16 @@ __device__ __forceinline__ void ga_eval8(const GemmActKernelArgs& a, const float
   }
 }
 // Eight 16-bit elements of which `valid` exist; the others are 0 and not read.
-__device__ __forceinline__ uint4 ga_load8(const void* p, int64_t valid) {
-  if (valid >= 8) return *static_cast<const uint4*>(p);
+__device__ __forceinline__ uint4 ga_load_any8(const uint16_t* p, int64_t valid) {
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i < valid) w[i >> 1] |= (uint32_t)static_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+    if (i < valid) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 ga_load8(const void* p, int64_t valid) {   // on a 16-byte boundary
+  if (valid >= 8) return *static_cast<const uint4*>(p);
+  return ga_load_any8(static_cast<const uint16_t*>(p), valid);
 }
 __device__ __forceinline__ uint4 ga_load_bias8(const GemmActKernelArgs& a, int64_t m) {
   if (!a.bias) return make_uint4(0, 0, 0, 0);
@@ -324,16 +354,16 @@ __device__ __forceinline__ void ga_finish(const GemmActKernelArgs& a, int64_t r,
 struct GaTile {
   int rt, qt;
 };
-// Tiles are numbered in panels of GA_PANEL q tiles, inside a panel along q first: what runs at
+// Tiles are numbered in panels of a few q tiles, inside a panel along q first: what runs at
 // one time then shares few X and few Y tiles, which cuts what is pulled through L2.
 __device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int64_t tile) {
-  const int64_t per_panel = (int64_t)a.r_tiles * GA_PANEL;
+  const int64_t per_panel = (int64_t)a.r_tiles * a.panel;
   const int panel = (int)(tile / per_panel);
-  const int width = min(GA_PANEL, a.q_tiles - panel * GA_PANEL);
+  const int width = min(a.panel, a.q_tiles - panel * a.panel);
   const int64_t rest = tile - panel * per_panel;
   GaTile t;
   t.rt = (int)(rest / width);
-  t.qt = panel * GA_PANEL + (int)(rest % width);
+  t.qt = panel * a.panel + (int)(rest % width);
   return t;
 }
 
@@ -350,7 +380,8 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   volatile int* abort_flag = &ctl->abort_flag;
   constexpr int EW = GaShape<BN>::EPILOGUE_WARPS;
   constexpr int YROWS = BN / CG;                       // rows of Y this CTA loads
-  constexpr uint32_t TMEM_COLS = 2 * BN < 32 ? 32 : 2 * BN;
+  constexpr uint32_t TMEM_COLS = 2 * BN;
+  const int bn = BN == 64 ? a.bn : BN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = (CG == 2 || a.split > 1) ? cluster_rank() : 0;
   const int split = CG == 1 ? a.split : 1;
@@ -394,78 +425,85 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (CG == 2) cluster_sync();     // the other CTA's barriers are initialised, its columns allocated
   ga_fence_after();
   const uint32_t tmem_base = ctl->tmem_base;
+  // Everything above may run while the kernel before this one in the stream still does; nothing
+  // below may, operands, results and the status word being global memory.
+  pdl_wait();
+  pdl_launch();
 
+  // The two issuing warps run their loops whole and elect a lane for the instructions that one
+  // thread has to issue: inside a branch on the lane number the compiler cannot keep descriptors
+  // and addresses in uniform registers, and the four MMAs of a stage then took 350 clocks to issue.
   if (warp == 0) {
     // ------------------------------ producer ------------------------------
-    if (lane == 0) {
-      int s = 0, filled = 0;         // stage, and how many stages have been filled at all (capped)
-      uint32_t phase = 0;            // parity of the ring's round
-      bool ok = true;
-      for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
-        const GaTile t = ga_tile(a, tile);
-        const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
-        const int q0 = t.qt * BN + (CG == 2 ? (int)rank * YROWS : 0);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (filled == a.stages && !mbar_wait_bounded(&ctl->empty[s], phase ^ 1u, abort_flag)) {
-            if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_EMPTY_WAIT_TIMEOUT); }
-            ok = false;
-            break;
-          }
+    const uint64_t pol_x = ga_policy_stream(), pol_y = ga_policy_normal();
+    // how far one k block moves the first two coordinates of a box
+    const int xk0 = a.x_mn ? 0 : GA_BK, xk1 = a.x_mn ? GA_BK : 0;
+    const int yk0 = a.y_mn ? 0 : GA_BK, yk1 = a.y_mn ? GA_BK : 0;
+    int s = 0, filled = 0;           // stage, and how many stages have been filled at all (capped)
+    uint32_t phase = 0;              // parity of the ring's round
+    bool ok = true;
+    for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+      const GaTile t = ga_tile(a, tile);
+      const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
+      const int q0 = t.qt * bn + (CG == 2 ? (int)rank * YROWS : 0);
+      int x0 = a.x_mn == GA_MN_BOXES ? r0 : a.x_mn ? 0 : kb0 * GA_BK, x1 = a.x_mn ? kb0 * GA_BK : r0;
+      int y0 = a.y_mn == GA_MN_BOXES ? q0 : a.y_mn ? 0 : kb0 * GA_BK, y1 = a.y_mn ? kb0 * GA_BK : q0;
+      const int x2 = a.x_mn == GA_MN_BLOCKS ? r0 / 64 : 0, y2 = a.y_mn == GA_MN_BLOCKS ? q0 / 64 : 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (filled == a.stages && !warp_wait(&ctl->empty[s], phase ^ 1u, abort_flag)) {
+          if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_EMPTY_WAIT_TIMEOUT); }
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
           const uint32_t x = smem_u32(smem) + s * a.stage_bytes, y = x + GA_X_BYTES;
           uint32_t bar = smem_u32(&ctl->full[s]);
           if (CG == 2) bar = map_rank(bar, 0);
           if (CG == 1 || rank == 0) mbar_expect_tx(&ctl->full[s], a.stage_bytes * CG);
-          if (a.x_mn == GA_MN_BLOCKS) {
-            ga_load<CG>(x, &map_x, bar, 0, kb * GA_BK, r0 / 64);
-          } else if (a.x_mn) {
-            ga_load<CG>(x, &map_x, bar, r0, kb * GA_BK);
-            ga_load<CG>(x + 8192, &map_x, bar, r0 + 64, kb * GA_BK);
-          } else {
-            ga_load<CG>(x, &map_x, bar, kb * GA_BK, r0);
-          }
-          if (YROWS >= 64 && a.y_mn == GA_MN_BLOCKS) {
-            ga_load<CG>(y, &map_y, bar, 0, kb * GA_BK, q0 / 64);
-          } else if (a.y_mn) {
+          ga_load<CG>(x, &map_x, bar, pol_x, x0, x1, x2);
+          if (a.x_mn == GA_MN_BOXES) ga_load<CG>(x + 8192, &map_x, bar, pol_x, x0 + 64, x1, 0);
+          ga_load<CG>(y, &map_y, bar, pol_y, y0, y1, y2);
+          if (a.y_mn == GA_MN_BOXES) {
 #pragma unroll
-            for (int j = 0; j < (YROWS + 63) / 64; ++j) ga_load<CG>(y + j * 8192, &map_y, bar, q0 + j * 64, kb * GA_BK);
-          } else {
-            ga_load<CG>(y, &map_y, bar, kb * GA_BK, q0);
+            for (int j = 1; j < YROWS / 64; ++j) ga_load<CG>(y + j * 8192, &map_y, bar, pol_y, y0 + j * 64, y1, 0);
           }
-          if (filled < a.stages) ++filled;
-          if (++s == a.stages) { s = 0; phase ^= 1u; }
         }
+        x0 += xk0; x1 += xk1; y0 += yk0; y1 += yk1;
+        if (filled < a.stages) ++filled;
+        if (++s == a.stages) { s = 0; phase ^= 1u; }
       }
-      // Before shared memory is given up: every stage has been read by its MMAs (with CG == 2 the
-      // leader's commits arrive here too, so none may still be on its way), or, after an abort,
-      // every copy has landed.
-      for (int j = 0; j < filled; ++j) {
-        // the oldest stage first; `s` and `phase` are those of the next fill
-        int zero = 0;
-        const int q = filled < a.stages ? j : (s + j < a.stages ? s + j : s + j - a.stages);
-        const uint32_t parity = filled < a.stages || q < s ? phase : phase ^ 1u;
-        uint64_t* bar = (ok && !*abort_flag) ? &ctl->empty[q] : &ctl->full[q];
-        if (CG == 2 && rank != 0 && (!ok || *abort_flag)) break;   // its copies signal the leader
-        if (!mbar_wait_bounded(bar, parity, &zero)) {
-          *abort_flag = 1;
-          atomicExch(a.status, KERR_DRAIN_TIMEOUT);
-          break;
-        }
+    }
+    // Before shared memory is given up: every stage has been read by its MMAs (with CG == 2 the
+    // leader's commits arrive here too, so none may still be on its way), or, after an abort,
+    // every copy has landed.
+    for (int j = 0; j < filled; ++j) {
+      // the oldest stage first; `s` and `phase` are those of the next fill
+      int zero = 0;
+      const int q = filled < a.stages ? j : (s + j < a.stages ? s + j : s + j - a.stages);
+      const uint32_t parity = filled < a.stages || q < s ? phase : phase ^ 1u;
+      const bool clean = __all_sync(0xffffffffu, ok && !*abort_flag);
+      if (CG == 2 && rank != 0 && !clean) break;   // its copies signal the leader
+      if (!warp_wait(clean ? &ctl->empty[q] : &ctl->full[q], parity, &zero)) {
+        *abort_flag = 1;
+        atomicExch(a.status, KERR_DRAIN_TIMEOUT);
+        break;
       }
     }
   } else if (warp == 1) {
     // ------------------------------ MMA issuer ------------------------------
-    if (lane == 0 && (CG == 1 || rank == 0)) {
+    if (CG == 1 || rank == 0) {
       const uint32_t fmt = a.bf16 ? 1u : 0u;
       const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a.x_mn ? 1u << 15 : 0u) | (a.y_mn ? 1u << 16 : 0u) |
-                             ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
-      const uint64_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
+                             ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+      const uint32_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
+      const uint64_t x_desc = ga_desc(smem_u32(smem), a.x_mn), y_desc = ga_desc(smem_u32(smem) + GA_X_BYTES, a.y_mn);
       int s = 0;
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
       for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
         const int buf = local & 1;
-        if (local >= 2 && !mbar_wait_bounded(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
+        if (local >= 2 && !warp_wait(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
           if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
           ok = false;
           break;
@@ -473,28 +511,31 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         ga_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(buf * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait_bounded(&ctl->full[s], phase, abort_flag)) {
+          if (!warp_wait(&ctl->full[s], phase, abort_flag)) {
             if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_FULL_WAIT_TIMEOUT); }
             ok = false;
             break;
           }
           ga_fence_after();
-          const uint32_t x = smem_u32(smem) + s * a.stage_bytes;
-          const uint64_t dx = ga_desc(x, a.x_mn), dy = ga_desc(x + GA_X_BYTES, a.y_mn);
+          if (elect_one()) {
+            const uint64_t dx = x_desc + (uint32_t)(s * (a.stage_bytes >> 4)), dy = y_desc + (uint32_t)(s * (a.stage_bytes >> 4));
 #pragma unroll
-          for (int j = 0; j < GA_BK / 16; ++j)
-            ga_mma<CG>(d, dx + j * x_step, dy + j * y_step, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
-          ga_commit<CG>(&ctl->empty[s]);
+            for (int j = 0; j < GA_BK / 16; ++j)
+              ga_mma<CG>(d, dx + j * x_step, dy + j * y_step, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
+            ga_commit<CG>(&ctl->empty[s]);
+          }
+          __syncwarp();
           if (++s == a.stages) { s = 0; phase ^= 1u; }
         }
-        if (ok) ga_commit<CG>(&ctl->acc_full[buf]);
+        if (ok && elect_one()) ga_commit<CG>(&ctl->acc_full[buf]);
+        __syncwarp();
       }
     }
   } else {
     // ------------------------------ epilogue ------------------------------
     const int quad = warp & 3, part = (warp - 2) >> 2;   // lanes of tensor memory; share of the columns
-    constexpr int W = QC && BN >= 32 ? 32 : 16;
-    constexpr int PART_COLS = BN / (EW / 4);
+    constexpr int W = QC ? 32 : 16;
+    const int part_cols = bn / (EW / 4);
     int local = 0;
     bool ok = true;
     for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
@@ -507,8 +548,8 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       }
       ga_fence_after();
       const int64_t r = (int64_t)t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32 + lane;
-      const int64_t q = (int64_t)t.qt * BN + part * PART_COLS;
-      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * PART_COLS);
+      const int64_t q = (int64_t)t.qt * bn + part * part_cols;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * part_cols);
       if constexpr (QC) {
         if (a.stage_out) {
           // 64 columns x 32 rows at a time through this warp's staging buffers (128-byte rows,
@@ -519,7 +560,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           const int r_first = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32;
           const bool row_in = r < a.N;
 #pragma unroll 1
-          for (int c = 0; c < PART_COLS; c += 64) {
+          for (int c = 0; c < part_cols; c += 64) {
             if (q + c >= a.M) break;
             if (lane == 0) ga_store_wait_read();
             __syncwarp();
@@ -558,7 +599,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
       }
 #pragma unroll 1
-      for (int c = 0; c < PART_COLS && !(QC && a.stage_out); c += W) {
+      for (int c = 0; c < part_cols && !(QC && a.stage_out); c += W) {
         float v[W];
         ga_tmem_ld<W>(taddr + c, v);
         if (a.kblocks == 0) {
@@ -567,7 +608,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
         }
         if (split > 1) {
           // column-major FP32 in the operand ring, which nothing reads any more
-          float* stage = reinterpret_cast<float*>(smem) + (part * PART_COLS + c) * 128 + quad * 32 + lane;
+          float* stage = reinterpret_cast<float*>(smem) + (part * part_cols + c) * 128 + quad * 32 + lane;
 #pragma unroll
           for (int j = 0; j < W; ++j) stage[j * 128] = v[j];
         } else {
@@ -593,24 +634,30 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const int row = e & 127, part = e >> 7;
       const GaTile t = ga_tile(a, first_tile);
       const int64_t r = (int64_t)t.rt * 128 + row;
-      const int cols = BN / split;                    // columns of this CTA
-      auto sum_run = [&](auto width) {
-        constexpr int W = decltype(width)::value;
-        for (int c = part * W; c < cols; c += W * (EW / 4)) {
-          const int col = (int)rank * cols + c;
-          float v[W];
+      const int cols = bn / split;                    // columns of this CTA
+      constexpr int W = QC ? 8 : 2;
+      for (int c = part * W; c < cols; c += W * (EW / 4)) {
+        const int col = (int)rank * cols + c;
+        if (!QC && (int64_t)t.qt * bn + col >= a.N) break;
+        const uint32_t own = smem_u32(smem) + (uint32_t)(col * 128 + row) * 4;
+        float p[8][W];
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[j] = 0.0f;
-          for (int s = 0; s < split; ++s) {
-            const uint32_t base = map_rank(smem_u32(smem) + (uint32_t)(col * 128 + row) * 4, s);
+        for (int s = 0; s < 8; ++s) {
+          const uint32_t base = map_rank(own, s < split ? s : 0);
 #pragma unroll
-            for (int j = 0; j < W; ++j) v[j] += ld_cluster(base + j * 512);
-          }
-          ga_finish<QC, W>(a, r, (int64_t)t.qt * BN + col, v);
+          for (int j = 0; j < W; ++j)
+            if (s < split) p[s][j] = ld_cluster(base + j * 512);
         }
-      };
-      if (QC || cols >= 8) sum_run(ActC<8>());
-      else sum_run(ActC<2>());
+        float v[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          v[j] = p[0][j];
+#pragma unroll
+          for (int s = 1; s < 8; ++s)
+            if (s < split) v[j] += p[s][j];
+        }
+        ga_finish<QC, W>(a, r, (int64_t)t.qt * bn + col, v);
+      }
     }
     __syncwarp();
     cluster_sync();      // nobody leaves while its shared memory is still read
@@ -629,18 +676,31 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ------------------------------------------------------------------ copy to an aligned layout
-// Column `blockIdx.y`-th of a len x cols matrix at any 2-byte address and leading dimension to a
-// buffer whose columns start on 16-byte boundaries, so that TMA can read it. A thread makes one
-// aligned group of eight; in the middle of a column it takes the two aligned 16-byte words that
-// the group straddles and shifts them together, so both sides move at full width.
-__global__ void __launch_bounds__(256)
-align_copy_kernel(const uint16_t* __restrict__ src, int64_t ld_src, uint16_t* __restrict__ dst, int64_t ld_dst,
-                  int64_t len, int64_t cols) {
-  const int64_t groups = (len + 7) / 8;
-  const int64_t total = groups * cols;
+// A len x cols matrix at any 2-byte address and leading dimension, copied to a buffer whose columns
+// start on 16-byte boundaries, so that TMA can read it; up to two matrices in a launch. A thread
+// makes one aligned group of eight; in the middle of a column it takes the two aligned 16-byte
+// words that the group straddles and shifts them together, so both sides move at full width.
+struct AlignCopy {
+  const uint16_t* src;
+  uint16_t* dst;
+  int64_t ld_src, ld_dst, len, cols;
+};
+struct AlignCopies {
+  AlignCopy m[2];
+  int64_t groups[2];   // of eight elements, in a matrix
+};
+
+__global__ void __launch_bounds__(256) align_copy_kernel(const __grid_constant__ AlignCopies c) {
+  pdl_wait();
+  pdl_launch();
+  const int64_t total = c.groups[0] + c.groups[1];
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t col = i / groups, g = i - col * groups;
-    const uint16_t* s = src + col * ld_src + g * 8;
+    const bool second = i >= c.groups[0];
+    const AlignCopy& m = c.m[second ? 1 : 0];
+    const int64_t j = second ? i - c.groups[0] : i;
+    const int64_t groups = m.ld_dst >> 3;
+    const int64_t col = j / groups, g = j - col * groups;
+    const uint16_t* s = m.src + col * m.ld_src + g * 8;
     uint4 o;
     if (g > 0 && g + 2 < groups) {
       const int shift = (int)(reinterpret_cast<uintptr_t>(s) & 15) * 8;   // bits
@@ -650,22 +710,16 @@ align_copy_kernel(const uint16_t* __restrict__ src, int64_t ld_src, uint16_t* __
       const int word = shift >> 5, bits = shift & 31;
       uint32_t q[5];
 #pragma unroll
-      for (int j = 0; j < 5; ++j)
-        q[j] = word == 0 ? w[j] : word == 1 ? w[j + 1] : word == 2 ? w[j + 2] : w[j + 3 < 8 ? j + 3 : 7];
+      for (int k = 0; k < 5; ++k)
+        q[k] = word == 0 ? w[k] : word == 1 ? w[k + 1] : word == 2 ? w[k + 2] : w[k + 3 < 8 ? k + 3 : 7];
       o.x = __funnelshift_r(q[0], q[1], bits);
       o.y = __funnelshift_r(q[1], q[2], bits);
       o.z = __funnelshift_r(q[2], q[3], bits);
       o.w = __funnelshift_r(q[3], q[4], bits);
     } else {
-      uint16_t e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = g * 8 + j < len ? s[j] : (uint16_t)0;
-      o.x = e[0] | (uint32_t)e[1] << 16;
-      o.y = e[2] | (uint32_t)e[3] << 16;
-      o.z = e[4] | (uint32_t)e[5] << 16;
-      o.w = e[6] | (uint32_t)e[7] << 16;
+      o = ga_load_any8(s, m.len - g * 8);
     }
-    *reinterpret_cast<uint4*>(dst + col * ld_dst + g * 8) = o;
+    *reinterpret_cast<uint4*>(m.dst + col * m.ld_dst + g * 8) = o;
   }
 }
 
@@ -760,6 +814,29 @@ inline bool vec16(const void* p, int64_t ld) {
 // ------------------------------------------------------------------ choice of a variant
 namespace {
 
+// Launch with programmatic stream serialization (the kernel waits with pdl_wait before it touches
+// global memory), in clusters of `cluster` blocks.
+template <typename... P, typename... Q>
+cudaError_t launch_dependent(void (*kernel)(P...), int grid, int threads, int smem, int cluster, cudaStream_t stream,
+                             Q&&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Q>(args)...);
+}
+
 // One way to run a product: orientation, tile, split of k.
 struct GaPlan {
   bool qc;
@@ -796,7 +873,7 @@ GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
   };
   const int64_t kb = (K + GA_BK - 1) / GA_BK;
   for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
-    for (int bn = qc ? 64 : 16; bn <= 256; bn *= 2) {
+    for (int bn = qc ? 64 : 16; bn <= 256; bn = bn < 64 ? bn + 16 : bn * 2) {
       if (qc && bn >= 128) consider({true, bn, 2, 1});
       if (!qc && bn == 256) consider({false, 256, 2, 1});
       if (bn <= 128)
@@ -809,10 +886,12 @@ GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
 template <int BN, int CG, bool QC>
 cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaStream_t stream) {
   constexpr int YROWS = BN / CG;
-  const int y_bytes = (a.y_mn ? std::max(YROWS, 64) : YROWS) * 128;
+  const int y_bytes = (a.y_mn || BN != 64 ? YROWS : a.bn) * 128;
   a.stage_bytes = GA_X_BYTES + y_bytes;
   const int staging = a.stage_out ? GaShape<BN>::EPILOGUE_WARPS * (a.pre ? 8192 : 4096) : 0;
-  a.stages = std::min(GA_MAX_STAGES, (GA_SMEM - staging) / a.stage_bytes);
+  int budget = GA_SMEM - staging;
+  if (BN == 64) budget = 108 * 1024 - staging;
+  a.stages = std::min(GA_MAX_STAGES, budget / a.stage_bytes);
   int smem = a.stages * a.stage_bytes + staging;
   if (a.split > 1) smem = std::max(smem, BN * 128 * 4);
   smem += 1024;
@@ -828,22 +907,10 @@ cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaSt
   }
   const int group = CG * a.split;
   int64_t grid = a.tiles * group;
-  if (a.split == 1) grid = std::min<int64_t>(grid, GA_SMS / CG * CG);
+  if (a.split == 1) grid = std::min<int64_t>(grid, (BN == 64 ? 2 * GA_SMS : GA_SMS) / CG * CG);
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(GaShape<BN>::THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = group;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = group > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], maps[3], a);
+  return launch_dependent(kernel, (int)grid, GaShape<BN>::THREADS, smem, group, stream, maps[0], maps[1], maps[2], maps[3],
+                          a);
 }
 
 // Whether TMA can read a stored operand of `cols` columns in place.
@@ -868,23 +935,28 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   const int64_t b_rows = p.tb ? p.N : p.K, b_cols = p.tb ? p.K : p.N;
   if (k_work) {
     char* s = static_cast<char*>(scratch);
-    auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) -> cudaError_t {
+    AlignCopies c;
+    memset(&c, 0, sizeof(c));
+    int n = 0;
+    auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
       const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
       const int64_t ld8 = (rows + 7) / 8 * 8;
-      if (bytes == 0) {
-        if (cols <= 1) ld = ld8;
-        return cudaSuccess;
+      if (bytes > 0) {
+        c.m[n] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(s), ld, ld8, rows, cols};
+        c.groups[n++] = ld8 / 8 * cols;
+        q = s;
+        ld = ld8;
+        s += bytes;
+      } else if (cols <= 1) {
+        ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
       }
-      const int64_t blocks = std::min<int64_t>((ld8 / 8 * cols + 255) / 256, GA_SMS * 16);
-      align_copy_kernel<<<(int)blocks, 256, 0, stream>>>(static_cast<const uint16_t*>(q), ld,
-                                                         reinterpret_cast<uint16_t*>(s), ld8, rows, cols);
-      q = s;
-      ld = ld8;
-      s += bytes;
-      return cudaGetLastError();
     };
-    PL_CUDA(in_reach(A, ldA, a_rows, a_cols));
-    PL_CUDA(in_reach(B, ldB, b_rows, b_cols));
+    in_reach(A, ldA, a_rows, a_cols);
+    in_reach(B, ldB, b_rows, b_cols);
+    if (n > 0) {
+      const int64_t blocks = std::min<int64_t>((c.groups[0] + c.groups[1] + 255) / 256, GA_SMS * 16);
+      PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, c));
+    }
   }
   auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
   const bool vec = vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) &&
@@ -901,11 +973,15 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   a.status = status;
   a.kblocks = (p.K + GA_BK - 1) / GA_BK;
   a.split = v.split;
+  a.bn = v.bn;
   const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
   const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
   a.tiles = r_tiles * q_tiles;
   a.r_tiles = (int32_t)r_tiles;
   a.q_tiles = (int32_t)q_tiles;
+  // A panel's share of Y is what L2 is to hold on to while X streams past: about 32 MB. At
+  // 8192^3 8 tiles of 256 rows are 850 us, 4 or 16 of them 880; at k = 4096 16 are 850 and 8 865.
+  a.panel = (int32_t)std::min<int64_t>(16, std::max<int64_t>(4, (32 << 20) / ((int64_t)v.bn * std::max(p.K, 1) * 2)));
   // op(A) is stored with k contiguous if it is a transpose, op(B) if it is not
   const bool a_k = p.ta != 0, b_k = p.tb == 0;
   const int yrows = v.bn / v.cg, xrows = 128;
@@ -929,9 +1005,7 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   }
   cudaError_t e = cudaErrorInvalidValue;
 #define GA_CASE(BN, CG, QC) \
-  if (v.bn == BN && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, a, stream);
-  GA_CASE(16, 1, false)
-  GA_CASE(32, 1, false)
+  if ((BN == 64 ? v.bn <= 64 : v.bn == BN) && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, a, stream);
   GA_CASE(64, 1, false)
   GA_CASE(128, 1, false)
   GA_CASE(256, 2, false)
