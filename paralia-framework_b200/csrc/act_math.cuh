@@ -26,16 +26,47 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
-// 1 / (1 + exp(-x)) for x >= -80: below that the caller clamps, since exp(-x) leaves the range
-// of the fast division.
-__device__ __forceinline__ float sigmoid_f32(float x) {
-  return __fdividef(1.0f, 1.0f + __expf(-x));
+// 2^x and 1/x of the special-function unit, two units in the last place or so; results below
+// 2^-126 are 0. The plain intrinsics wrap them in code for subnormal numbers, which nothing here
+// needs and which the epilogue of a product pays for 32768 times a tile.
+__device__ __forceinline__ float exp2_f32(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_f32(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float GELU_C = 0.7978845608028654f;    // sqrt(2/pi)
 constexpr float GELU_A = 0.044715f;
-constexpr float INV_SQRT2 = 0.7071067811865476f;
 constexpr float INV_SQRT_2PI = 0.3989422804014327f;
+
+// 1 / (1 + 2^y); 0 from y = 128 on.
+__device__ __forceinline__ float sigmoid_exp2(float y) { return rcp_f32(1.0f + exp2_f32(y)); }
+
+// Phi(-x) = erfc(x / sqrt(2)) / 2 for x >= 0, by the Chebyshev fit of erfc with a relative error below
+// 1.2e-7 everywhere (Press et al., Numerical Recipes, "erfcc"): erfc(w) = t exp(-w^2 + P(t)),
+// t = 1 / (1 + w/2). The factors log2(e) of the exponent and 1/2 of the result are in the constants.
+__device__ __forceinline__ float normal_tail(float x) {
+  constexpr float L = LOG2E;
+  const float t = rcp_f32(fmaf(0.35355339059327373f, x, 1.0f));
+  float p = 0.17087277f * L;
+  p = fmaf(p, t, -0.82215223f * L);
+  p = fmaf(p, t, 1.48851587f * L);
+  p = fmaf(p, t, -1.13520398f * L);
+  p = fmaf(p, t, 0.27886807f * L);
+  p = fmaf(p, t, -0.18628806f * L);
+  p = fmaf(p, t, 0.09678418f * L);
+  p = fmaf(p, t, 0.37409196f * L);
+  p = fmaf(p, t, 1.00002368f * L);
+  p = fmaf(p, t, -1.26551223f * L - 1.0f);
+  const float w = 0.8493218002880191f * x;    // sqrt(log2(e) / 2): w^2 is the exponent to base 2
+  return t * exp2_f32(fmaf(-w, w, p));
+}
 
 // The three smooth activations vanish to the left faster than any 16-bit type resolves, so z
 // is clamped there: act(-inf) is then 0 and not inf * 0. A NaN stays a NaN throughout.
@@ -43,16 +74,17 @@ template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if (ACT == PARALIA_ACT_RELU) return z < 0.0f ? 0.0f : z;
   if (ACT == PARALIA_ACT_GELU) {
-    const float c = max_nan(z, -30.0f);
-    return 0.5f * c * erfcf(-c * INV_SQRT2);
+    const float c = max_nan(z, -30.0f), h = normal_tail(fabsf(c));
+    return c * (c > 0.0f ? 1.0f - h : h);
   }
   if (ACT == PARALIA_ACT_GELU_TANH) {
-    const float c = max_nan(z, -9.0f);    // 2u = -66 there
-    return c * sigmoid_f32(2.0f * GELU_C * c * fmaf(GELU_A * c, c, 1.0f));
+    constexpr float K1 = -2.0f * GELU_C * LOG2E, K2 = K1 * GELU_A;
+    const float c = max_nan(z, -9.0f);    // the exponent is 95 there
+    return c * sigmoid_exp2(c * fmaf(K2, c * c, K1));
   }
   if (ACT == PARALIA_ACT_SILU) {
     const float c = max_nan(z, -80.0f);
-    return c * sigmoid_f32(c);
+    return c * sigmoid_exp2(-LOG2E * c);
   }
   return z;
 }
@@ -63,36 +95,44 @@ __device__ __forceinline__ float act_slope(float z) {
   if (ACT == PARALIA_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (ACT == PARALIA_ACT_GELU) {
     const float c = min_nan(max_nan(z, -30.0f), 30.0f);
-    return fmaf(c * INV_SQRT_2PI, __expf(-0.5f * c * c), 0.5f * erfcf(-c * INV_SQRT2));
+    const float h = normal_tail(fabsf(c)), w = 0.8493218002880191f * c;
+    return fmaf(c * INV_SQRT_2PI, exp2_f32(-w * w), c > 0.0f ? 1.0f - h : h);
   }
   if (ACT == PARALIA_ACT_GELU_TANH) {
-    const float c = min_nan(max_nan(z, -9.0f), 9.0f);
-    const float q = GELU_A * c * c;
-    const float g = sigmoid_f32(2.0f * GELU_C * c * (1.0f + q));
-    return fmaf(2.0f * GELU_C * c * (1.0f + 3.0f * q), g * (1.0f - g), g);
+    constexpr float K1 = -2.0f * GELU_C * LOG2E, K2 = K1 * GELU_A;
+    const float c = min_nan(max_nan(z, -9.0f), 9.0f), q = c * c;
+    const float g = sigmoid_exp2(c * fmaf(K2, q, K1));
+    return fmaf(c * fmaf(6.0f * GELU_C * GELU_A, q, 2.0f * GELU_C), g * (1.0f - g), g);
   }
   if (ACT == PARALIA_ACT_SILU) {
     const float c = min_nan(max_nan(z, -80.0f), 80.0f);
-    const float g = sigmoid_f32(c);
+    const float g = sigmoid_exp2(-LOG2E * c);
     return fmaf(c * g, 1.0f - g, g);
   }
   return 1.0f;
 }
 
-// Run `f` with the activation as a compile-time constant: f(std::integral_constant<int, ACT>).
+// Run `f` with the activation, or with the activation and the element type, as compile-time
+// constants: f(IntC<ACT>()), f(IntC<ACT>(), IntC<BF16>()).
 template <int V>
-struct ActC {
+struct IntC {
   static constexpr int value = V;
 };
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F f) {
   switch (act) {
-    case PARALIA_ACT_RELU: f(ActC<PARALIA_ACT_RELU>()); break;
-    case PARALIA_ACT_GELU: f(ActC<PARALIA_ACT_GELU>()); break;
-    case PARALIA_ACT_GELU_TANH: f(ActC<PARALIA_ACT_GELU_TANH>()); break;
-    case PARALIA_ACT_SILU: f(ActC<PARALIA_ACT_SILU>()); break;
-    default: f(ActC<PARALIA_ACT_NONE>()); break;
+    case PARALIA_ACT_RELU: f(IntC<PARALIA_ACT_RELU>()); break;
+    case PARALIA_ACT_GELU: f(IntC<PARALIA_ACT_GELU>()); break;
+    case PARALIA_ACT_GELU_TANH: f(IntC<PARALIA_ACT_GELU_TANH>()); break;
+    case PARALIA_ACT_SILU: f(IntC<PARALIA_ACT_SILU>()); break;
+    default: f(IntC<PARALIA_ACT_NONE>()); break;
   }
+}
+
+template <typename F>
+__device__ __forceinline__ void with_act_type(int act, bool bf16, F f) {
+  if (bf16) with_act(act, [&](auto a) { f(a, IntC<1>()); });
+  else with_act(act, [&](auto a) { f(a, IntC<0>()); });
 }
 
 // One 16-bit element to and from FP32; `bf` tells BF16 from FP16.

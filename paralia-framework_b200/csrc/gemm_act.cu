@@ -63,7 +63,7 @@ struct GemmActKernelArgs {
   void* D;
   void* pre;
   int64_t ldC, ldD, ldPre;
-  int64_t tiles;
+  int32_t tiles;
   int32_t M, N;
   int32_t r_tiles, q_tiles;
   int32_t panel;                 // q tiles per panel of the tile numbering
@@ -114,9 +114,12 @@ __device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
@@ -221,28 +224,9 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, const uint32_t (&v)[4
 __device__ __forceinline__ void ga_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void ga_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-template <int W>
-__device__ __forceinline__ void ga_tmem_ld(uint32_t taddr, float (&v)[W]);
-template <>
-__device__ __forceinline__ void ga_tmem_ld<32>(uint32_t taddr, float (&v)[32]) {
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr)
-      : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-template <>
-__device__ __forceinline__ void ga_tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
+// Sixteen columns of this warp's 32 lanes of tensor memory, on their way; they are there after
+// ga_tmem_wait16, which ties the registers to the wait.
+__device__ __forceinline__ void ga_tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
       "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -250,30 +234,45 @@ __device__ __forceinline__ void ga_tmem_ld<16>(uint32_t taddr, float (&v)[16]) {
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void ga_tmem_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
 }
 
 // ------------------------------------------------------------------ epilogue
-// Eight neighbouring rows of one column of D: from sums, bias and C to packed D and Z.
-template <int ACT>
-__device__ __forceinline__ void ga_eval8(const GemmActKernelArgs& a, const float* v, const uint4& b, const uint4& c,
-                                         uint32_t (&d)[4], uint32_t (&z)[4]) {
-  const bool bf = a.bf16 != 0;
-  const uint32_t cv[4] = {c.x, c.y, c.z, c.w}, bv[4] = {b.x, b.y, b.z, b.w};
+// Eight neighbouring rows of one column of D. First Z from sums and bias, then D and Z packed.
+template <bool bf>
+__device__ __forceinline__ void ga_z8(const GemmActKernelArgs& a, const float* v, const uint4& b, float* z) {
+  const uint32_t bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 bb = unpack16(bv[i], bf), cc = unpack16(cv[i], bf);
-    const float z0 = fmaf(a.alpha, v[2 * i], bb.x), z1 = fmaf(a.alpha, v[2 * i + 1], bb.y);
-    z[i] = pack16(z0, z1, bf);
-    float d0 = act_value<ACT>(z0), d1 = act_value<ACT>(z1);
+    const float2 bb = unpack16(bv[i], bf);
+    z[2 * i] = fmaf(a.alpha, v[2 * i], bb.x);
+    z[2 * i + 1] = fmaf(a.alpha, v[2 * i + 1], bb.y);
+  }
+}
+template <int ACT, bool bf>
+__device__ __forceinline__ void ga_d8(const GemmActKernelArgs& a, const float* z, const uint4& c, uint32_t (&d)[4]) {
+  const uint32_t cv[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float d0 = act_value<ACT>(z[2 * i]), d1 = act_value<ACT>(z[2 * i + 1]);
     if (a.C) {
+      const float2 cc = unpack16(cv[i], bf);
       d0 = fmaf(a.beta, cc.x, d0);
       d1 = fmaf(a.beta, cc.y, d1);
     }
     d[i] = pack16(d0, d1, bf);
   }
+}
+template <bool bf>
+__device__ __forceinline__ void ga_pack8(const float* z, uint32_t (&p)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = pack16(z[2 * i], z[2 * i + 1], bf);
 }
 // Eight 16-bit elements of which `valid` exist; the others are 0 and not read.
 __device__ __forceinline__ uint4 ga_load_any8(const uint16_t* p, int64_t valid) {
@@ -288,21 +287,23 @@ __device__ __forceinline__ uint4 ga_load8(const void* p, int64_t valid) {   // o
   return ga_load_any8(static_cast<const uint16_t*>(p), valid);
 }
 __device__ __forceinline__ uint4 ga_load_bias8(const GemmActKernelArgs& a, int64_t m) {
-  if (!a.bias) return make_uint4(0, 0, 0, 0);
+  if (!a.bias || m >= a.M) return make_uint4(0, 0, 0, 0);
   return ga_load8(static_cast<const uint16_t*>(a.bias) + m, a.M - m);
 }
 __device__ __forceinline__ uint4 ga_load_c8(const GemmActKernelArgs& a, int64_t m, int64_t n) {
-  if (!a.C) return make_uint4(0, 0, 0, 0);
+  if (!a.C || m >= a.M) return make_uint4(0, 0, 0, 0);
   return ga_load8(static_cast<const uint16_t*>(a.C) + m + n * a.ldC, a.M - m);
 }
 
 // Rows m .. m+7 of column n of D (QC): acc -> D, pre.
-template <int ACT>
+template <int ACT, bool bf>
 __device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m, int64_t n, float* v) {
-  const bool bf = a.bf16 != 0;
   if (a.vec && m + 8 <= a.M) {
+    float zf[8];
     uint32_t z[4], d[4];
-    ga_eval8<ACT>(a, v, ga_load_bias8(a, m), ga_load_c8(a, m, n), d, z);
+    ga_z8<bf>(a, v, ga_load_bias8(a, m), zf);
+    ga_d8<ACT, bf>(a, zf, ga_load_c8(a, m, n), d);
+    ga_pack8<bf>(zf, z);
     if (a.pre) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.pre) + m + n * a.ldPre) = make_uint4(z[0], z[1], z[2], z[3]);
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.D) + m + n * a.ldD) = make_uint4(d[0], d[1], d[2], d[3]);
     return;
@@ -321,33 +322,114 @@ __device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m
 // W accumulator columns q0 .. q0+W-1 of lane row r.
 template <bool QC, int W>
 __device__ __forceinline__ void ga_finish(const GemmActKernelArgs& a, int64_t r, int64_t q0, float (&v)[W]) {
-  with_act(a.act, [&](auto t) {
+  with_act_type(a.act, a.bf16 != 0, [&](auto t, auto y) {
     constexpr int ACT = decltype(t)::value;
+    constexpr bool bf = decltype(y)::value != 0;
     if constexpr (QC) {
       if (r >= a.N) return;
 #pragma unroll
       for (int g = 0; g < W / 8; ++g)
-        if (q0 + 8 * g < a.M) ga_finish8<ACT>(a, q0 + 8 * g, r, &v[8 * g]);
+        if (q0 + 8 * g < a.M) ga_finish8<ACT, bf>(a, q0 + 8 * g, r, &v[8 * g]);
     } else {
       if (r >= a.M) return;
-      const bool bf = a.bf16 != 0;
       const float b = a.bias ? load16(a.bias, r, bf) : 0.0f;
-      float c[W];
+      uint16_t c[W];
       if (a.C) {
+        // all on their way before the first is used; past the last column the last one again
 #pragma unroll
-        for (int j = 0; j < W; ++j) c[j] = q0 + j < a.N ? load16(a.C, r + (q0 + j) * a.ldC, bf) : 0.0f;
+        for (int j = 0; j < W; ++j)
+          c[j] = static_cast<const uint16_t*>(a.C)[r + min(q0 + j, (int64_t)a.N - 1) * a.ldC];
       }
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        if (q0 + j >= a.N) break;
         const float z = fmaf(a.alpha, v[j], b);
-        if (a.pre) store16(a.pre, r + (q0 + j) * a.ldPre, z, bf);
         float d = act_value<ACT>(z);
-        if (a.C) d = fmaf(a.beta, c[j], d);
-        store16(a.D, r + (q0 + j) * a.ldD, d, bf);
+        if (a.C) d = fmaf(a.beta, load16(&c[j], 0, bf), d);
+        if (q0 + j < a.N) {
+          if (a.pre) store16(a.pre, r + (q0 + j) * a.ldPre, z, bf);
+          store16(a.D, r + (q0 + j) * a.ldD, d, bf);
+        }
       }
     }
   });
+}
+
+// One warp's share of a tile (QC): 32 columns of D, `cols` rows from q on, a multiple of 64. Once Z has
+// been made of the sums of 16 rows, the next 16 are fetched under the rest of the work on these. 64
+// rows at a time leave through this warp's staging buffer (128-byte lines, swizzled as the tensor map
+// says) by TMA: whole lines, edges clipped by the map, the store under the next arithmetic. The loop
+// is not unrolled: with ten variants and eight warps out of step the instruction cache is what an
+// unrolled one waits for (8192 x 8192 x 1024 with tanh-GELU: 174 us unrolled by four).
+template <int ACT, bool bf>
+__device__ __forceinline__ void ga_staged_tile(const GemmActKernelArgs& a, const CUtensorMap* map_d,
+                                               const CUtensorMap* map_pre, uint32_t taddr, uint32_t out, int q,
+                                               int r_first, int cols, int lane) {
+  const uint32_t row = out + lane * 128;
+  const int64_t n = min((int64_t)r_first + lane, (int64_t)a.N - 1);   // a column that exists; its copy is cut off
+  const int last = min(cols, ((a.M - q + 63) / 64) * 64);              // 64 rows of which none exists are left out
+  if (last <= 0) return;
+  uint32_t v[16];
+  uint4 c0 = ga_load_c8(a, q, n), c1 = ga_load_c8(a, (int64_t)q + 8, n);
+  uint4 b0 = ga_load_bias8(a, q), b1 = ga_load_bias8(a, (int64_t)q + 8);
+  ga_tmem_ld16(taddr, v);
+#pragma unroll 1
+  for (int at = 0; at < last; at += 16) {
+    ga_tmem_wait16(v);
+    float x[16], z[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = a.kblocks == 0 ? 0.0f : __uint_as_float(v[e]);
+    ga_z8<bf>(a, x, b0, z);
+    ga_z8<bf>(a, x + 8, b1, z + 8);
+    const uint4 cx0 = c0, cx1 = c1;
+    if (at + 16 < last) {
+      ga_tmem_ld16(taddr + at + 16, v);
+      const int64_t m = (int64_t)q + at + 16;
+      c0 = ga_load_c8(a, m, n);
+      c1 = ga_load_c8(a, m + 8, n);
+      b0 = ga_load_bias8(a, m);
+      b1 = ga_load_bias8(a, m + 8);
+    }
+    if ((at & 63) == 0) {
+      if (lane == 0) ga_store_wait_read();
+      __syncwarp();
+    }
+    uint32_t o[4];
+    const uint32_t to0 = row + (((at & 63) >> 3) ^ (lane & 7)) * 16, to1 = row + ((((at & 63) >> 3) + 1) ^ (lane & 7)) * 16;
+    ga_d8<ACT, bf>(a, z, cx0, o);
+    st_shared16(to0, o);
+    ga_d8<ACT, bf>(a, z + 8, cx1, o);
+    st_shared16(to1, o);
+    if (a.pre) {
+      ga_pack8<bf>(z, o);
+      st_shared16(to0 + 4096, o);
+      ga_pack8<bf>(z + 8, o);
+      st_shared16(to1 + 4096, o);
+    }
+    if ((at & 63) == 48) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0 && r_first < a.N) {
+        ga_store(map_d, out, q + at - 48, r_first);
+        if (a.pre) ga_store(map_pre, out + 4096, q + at - 48, r_first);
+        ga_store_commit();
+      }
+    }
+  }
+}
+
+// Asks L2 for the rows m0 .. m0+rows-1 of the bias and of `cols` columns of C from n0 on. The epilogue's
+// own loads come late and few at a time, each with the latency of where the line then is.
+template <int THREADS>
+__device__ __forceinline__ void ga_prefetch_inputs(const GemmActKernelArgs& a, int64_t m0, int rows, int64_t n0, int cols) {
+  const int e = threadIdx.x - 64, lines = (rows + 63) / 64;
+  if (a.bias && e < lines && m0 + e * 64 < a.M)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.bias) + m0 + e * 64));
+  if (!a.C) return;
+  for (int i = e; i < lines * cols; i += THREADS) {
+    const int64_t m = m0 + (i % lines) * 64, n = n0 + i / lines;
+    if (m < a.M && n < a.N)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.C) + m + n * a.ldC));
+  }
 }
 
 // ------------------------------------------------------------------ kernel
@@ -356,19 +438,18 @@ struct GaTile {
 };
 // Tiles are numbered in panels of a few q tiles, inside a panel along q first: what runs at
 // one time then shares few X and few Y tiles, which cuts what is pulled through L2.
-__device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int64_t tile) {
-  const int64_t per_panel = (int64_t)a.r_tiles * a.panel;
-  const int panel = (int)(tile / per_panel);
-  const int width = min(a.panel, a.q_tiles - panel * a.panel);
-  const int64_t rest = tile - panel * per_panel;
+__device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int tile) {
+  const uint32_t per_panel = (uint32_t)a.r_tiles * (uint32_t)a.panel;
+  const uint32_t panel = (uint32_t)tile / per_panel, rest = (uint32_t)tile - panel * per_panel;
+  const uint32_t width = min((uint32_t)a.panel, (uint32_t)a.q_tiles - panel * (uint32_t)a.panel);
   GaTile t;
   t.rt = (int)(rest / width);
-  t.qt = panel * a.panel + (int)(rest % width);
+  t.qt = (int)(panel * (uint32_t)a.panel + rest - (uint32_t)t.rt * width);
   return t;
 }
 
 template <int BN, int CG, bool QC>
-__global__ void __launch_bounds__(GaShape<BN>::THREADS, 1)
+__global__ void __launch_bounds__(GaShape<BN>::THREADS, BN == 64 ? 2 : 1)
 gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
                 const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_pre,
                 const __grid_constant__ GemmActKernelArgs a) {
@@ -381,12 +462,12 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   constexpr int EW = GaShape<BN>::EPILOGUE_WARPS;
   constexpr int YROWS = BN / CG;                       // rows of Y this CTA loads
   constexpr uint32_t TMEM_COLS = 2 * BN;
-  const int bn = BN == 64 ? a.bn : BN;
+  const int bn = BN == 64 && !QC ? a.bn : BN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = (CG == 2 || a.split > 1) ? cluster_rank() : 0;
   const int split = CG == 1 ? a.split : 1;
   const int group = CG * split;                        // CTAs that share a tile
-  const int64_t first_tile = blockIdx.x / group, tile_step = gridDim.x / group;
+  const int first_tile = blockIdx.x / group, tile_step = gridDim.x / group;
   // this CTA's run of k blocks
   const int kb0 = split > 1 ? (int)((int64_t)a.kblocks * rank / split) : 0;
   const int kb1 = split > 1 ? (int)((int64_t)a.kblocks * (rank + 1) / split) : a.kblocks;
@@ -442,7 +523,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     int s = 0, filled = 0;           // stage, and how many stages have been filled at all (capped)
     uint32_t phase = 0;              // parity of the ring's round
     bool ok = true;
-    for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+    for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
       const GaTile t = ga_tile(a, tile);
       const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
       const int q0 = t.qt * bn + (CG == 2 ? (int)rank * YROWS : 0);
@@ -501,7 +582,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+      for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
         const int buf = local & 1;
         if (local >= 2 && !warp_wait(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
           if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
@@ -534,13 +615,21 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else {
     // ------------------------------ epilogue ------------------------------
     const int quad = warp & 3, part = (warp - 2) >> 2;   // lanes of tensor memory; share of the columns
-    constexpr int W = QC ? 32 : 16;
+    constexpr int W = 16;
     const int part_cols = bn / (EW / 4);
     int local = 0;
     bool ok = true;
-    for (int64_t tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+    for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
       const int buf = local & 1;
       const GaTile t = ga_tile(a, tile);
+      {
+        // what the epilogue will read, into L2 while the product runs
+        const int q_cols = bn / split;
+        const int64_t r_first = (int64_t)t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
+        const int64_t q_first = (int64_t)t.qt * bn + (split > 1 ? (int)rank * q_cols : 0);
+        ga_prefetch_inputs<EW * 32>(a, QC ? q_first : r_first, QC ? q_cols : 128, QC ? r_first : q_first,
+                                    QC ? 128 : q_cols);
+      }
       if (!mbar_wait_bounded(&ctl->acc_full[buf], (uint32_t)((local >> 1) & 1), abort_flag)) {
         if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
         ok = false;
@@ -552,56 +641,22 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * part_cols);
       if constexpr (QC) {
         if (a.stage_out) {
-          // 64 columns x 32 rows at a time through this warp's staging buffers (128-byte rows,
-          // swizzled as the tensor map says), written out by TMA: whole lines leave, edges are
-          // clipped by the map, and the store runs under the next columns' arithmetic
           const uint32_t out = smem_u32(smem) + a.stages * a.stage_bytes + (warp - 2) * (a.pre ? 8192 : 4096);
-          const uint32_t row = out + lane * 128;
           const int r_first = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32;
-          const bool row_in = r < a.N;
-#pragma unroll 1
-          for (int c = 0; c < part_cols; c += 64) {
-            if (q + c >= a.M) break;
-            if (lane == 0) ga_store_wait_read();
-            __syncwarp();
-#pragma unroll 1
-            for (int h = 0; h < 64; h += 32) {
-              uint4 cc[4];
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-                cc[g] = row_in ? ga_load_c8(a, q + c + h + 8 * g, r) : make_uint4(0, 0, 0, 0);
-              float v[32];
-              ga_tmem_ld<32>(taddr + c + h, v);
-              if (a.kblocks == 0) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-              }
-              with_act(a.act, [&](auto k) {
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                  const int64_t m = q + c + h + 8 * g;
-                  uint32_t d[4], z[4];
-                  ga_eval8<decltype(k)::value>(a, &v[8 * g], ga_load_bias8(a, m), cc[g], d, z);
-                  const uint32_t at = row + (((h >> 3) + g) ^ (lane & 7)) * 16;
-                  st_shared16(at, d);
-                  if (a.pre) st_shared16(at + 4096, z);
-                }
-              });
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0 && r_first < a.N) {
-              ga_store(&map_d, out, (int)(q + c), r_first);
-              if (a.pre) ga_store(&map_pre, out + 4096, (int)(q + c), r_first);
-              ga_store_commit();
-            }
-          }
+          with_act_type(a.act, a.bf16 != 0, [&](auto k, auto y) {
+            ga_staged_tile<decltype(k)::value, decltype(y)::value != 0>(a, &map_d, &map_pre, taddr, out, (int)q, r_first,
+                                                                        part_cols, lane);
+          });
         }
       }
 #pragma unroll 1
       for (int c = 0; c < part_cols && !(QC && a.stage_out); c += W) {
+        uint32_t raw[W];
+        ga_tmem_ld16(taddr + c, raw);
+        ga_tmem_wait16(raw);
         float v[W];
-        ga_tmem_ld<W>(taddr + c, v);
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = __uint_as_float(raw[j]);
         if (a.kblocks == 0) {
 #pragma unroll
           for (int j = 0; j < W; ++j) v[j] = 0.0f;   // the accumulator was never written
@@ -611,8 +666,14 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
           float* stage = reinterpret_cast<float*>(smem) + (part * part_cols + c) * 128 + quad * 32 + lane;
 #pragma unroll
           for (int j = 0; j < W; ++j) stage[j * 128] = v[j];
-        } else {
-          ga_finish<QC, W>(a, r, q + c, v);
+        } else if constexpr (!QC) {
+#pragma unroll 1
+          for (int g = 0; g < W; g += 8) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = g == 0 ? v[j] : v[8 + j];
+            ga_finish<QC, 8>(a, r, q + c + g, x);
+          }
         }
       }
       ga_fence_before();
@@ -629,34 +690,34 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     // ------------------------------ sum over the cluster ------------------------------
     __syncwarp();
     cluster_sync();
-    if (warp >= 2 && !*abort_flag) {
-      const int e = threadIdx.x - 64;                 // 0 .. EW * 32 - 1
-      const int row = e & 127, part = e >> 7;
-      const GaTile t = ga_tile(a, first_tile);
-      const int64_t r = (int64_t)t.rt * 128 + row;
+    if (warp >= 2) {
+      // A warp sums one column of this CTA's share at a time, a lane four rows of it: 512 contiguous
+      // bytes from each CTA. The sums replace this CTA's own share, which nobody else reads.
       const int cols = bn / split;                    // columns of this CTA
+      const GaTile t = ga_tile(a, first_tile);
+      float* own = reinterpret_cast<float*>(smem) + (int)rank * cols * 128;
+      // columns that exist (QC: all, the others are cut off later)
+      const int used = QC ? cols : (int)min((int64_t)cols, max((int64_t)0, a.N - ((int64_t)t.qt * bn + rank * cols)));
+      for (int c = warp - 2; c < used; c += EW) {
+        const uint32_t at = smem_u32(own + c * 128 + lane * 4);
+        float4 p[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          if (s < split) p[s] = ld_cluster(map_rank(at, s));
+        float4 v = p[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+          if (s < split) { v.x += p[s].x; v.y += p[s].y; v.z += p[s].z; v.w += p[s].w; }
+        *reinterpret_cast<float4*>(own + c * 128 + lane * 4) = v;
+      }
+      named_bar_sync(1, EW * 32);
+      const int row = (threadIdx.x - 64) & 127, part = (threadIdx.x - 64) >> 7;
       constexpr int W = QC ? 8 : 2;
-      for (int c = part * W; c < cols; c += W * (EW / 4)) {
-        const int col = (int)rank * cols + c;
-        if (!QC && (int64_t)t.qt * bn + col >= a.N) break;
-        const uint32_t own = smem_u32(smem) + (uint32_t)(col * 128 + row) * 4;
-        float p[8][W];
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          const uint32_t base = map_rank(own, s < split ? s : 0);
-#pragma unroll
-          for (int j = 0; j < W; ++j)
-            if (s < split) p[s][j] = ld_cluster(base + j * 512);
-        }
+      for (int c = part * W; c < used; c += W * (EW / 4)) {
         float v[W];
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          v[j] = p[0][j];
-#pragma unroll
-          for (int s = 1; s < 8; ++s)
-            if (s < split) v[j] += p[s][j];
-        }
-        ga_finish<QC, W>(a, r, (int64_t)t.qt * bn + col, v);
+        for (int j = 0; j < W; ++j) v[j] = own[(c + j) * 128 + row];
+        ga_finish<QC, W>(a, (int64_t)t.rt * 128 + row, (int64_t)t.qt * bn + (int)rank * cols + c, v);
       }
     }
     __syncwarp();
@@ -742,10 +803,10 @@ __global__ void __launch_bounds__(AG_WARPS * 32) act_grad_kernel(const ActGradPr
   const int64_t row0 = (int64_t)blockIdx.x * AG_ROWS;
   const int64_t n_begin = (int64_t)blockIdx.y * cols;
   const int64_t n_end = min((int64_t)p.N, n_begin + cols);
-  const bool bf = p.bf16 != 0;
   float acc[8] = {};
-  with_act(p.act, [&](auto a) {
+  with_act_type(p.act, p.bf16 != 0, [&](auto a, auto y) {
     constexpr int ACT = decltype(a)::value;
+    constexpr bool bf = decltype(y)::value != 0;
     for (int64_t n = n_begin + warp; n < n_end; n += AG_WARPS) {
       if (VEC) {
         const int64_t m = row0 + lane * 8;
@@ -906,9 +967,8 @@ cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaSt
     configured[dev] = true;
   }
   const int group = CG * a.split;
-  int64_t grid = a.tiles * group;
+  int64_t grid = (int64_t)a.tiles * group;
   if (a.split == 1) grid = std::min<int64_t>(grid, (BN == 64 ? 2 * GA_SMS : GA_SMS) / CG * CG);
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
   return launch_dependent(kernel, (int)grid, GaShape<BN>::THREADS, smem, group, stream, maps[0], maps[1], maps[2], maps[3],
                           a);
 }
@@ -976,7 +1036,10 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   a.bn = v.bn;
   const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
   const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
-  a.tiles = r_tiles * q_tiles;
+  // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits
+  if (r_tiles * std::max<int64_t>(q_tiles, 16) * 8 > INT32_MAX)
+    return fail(PARALIA_ERR_UNSUPPORTED, "M = %d, N = %d: too many tiles", p.M, p.N);
+  a.tiles = (int32_t)(r_tiles * q_tiles);
   a.r_tiles = (int32_t)r_tiles;
   a.q_tiles = (int32_t)q_tiles;
   // A panel's share of Y is what L2 is to hold on to while X streams past: about 32 MB. At
