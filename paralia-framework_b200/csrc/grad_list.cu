@@ -3,9 +3,10 @@
 //
 // Both kernels are bound by HBM: one read of the list for the norm, one read and one write for
 // the scaling. The list travels in the kernel's parameters (no copy, nothing kept between
-// calls, capturable); it is cut into chunks of equal length, block b takes chunks b, b + grid,
-// ..., and a binary search over the tensors' first chunks finds the tensor of a chunk. The
-// order of every sum is a function of the list alone.
+// calls, capturable). It is cut into units of 2048 elements and block b of G takes the b-th of G
+// equal runs of units, so what a block has of one tensor is one contiguous span (chunks dealt out
+// in turn, with a search for the tensor of each, read 2 GB of BF16 in 365 us). The order of every
+// sum is a function of the list alone.
 //
 // Squares: of FP32 elements they are summed in FP64 throughout (a conversion and an FMA an
 // element, which the FP64 pipe keeps up with at HBM speed). Of 16-bit elements the eight of
@@ -16,6 +17,8 @@
 #include "grad_list.cuh"
 
 #include <algorithm>
+#include <cstring>
+#include <utility>
 
 #include "act_math.cuh"
 
@@ -23,27 +26,21 @@ namespace paralia {
 namespace {
 
 constexpr int GL_THREADS = 512;
+constexpr int GL_CHUNK = 8;      // units a block scales at most: four groups of eight for every thread
 
 template <int CAP>
 struct GradTable {
   int32_t count;
-  int32_t chunk;        // elements
-  int32_t chunk_begin;  // first chunk of this launch (chunk0 of the entries counts from there)
-  int32_t chunks;
+  int32_t units;        // of this launch (unit0 of the entries counts within it)
+  int32_t starts;       // first[s] = the tensor with unit  units * s / starts
+  uint16_t first[GL_NORM_BLOCKS];
   GradEntry e[CAP];
 };
 
-// Index of the tensor that holds chunk c.
-template <int CAP>
-__device__ __forceinline__ int find_tensor(const GradTable<CAP>& t, int c) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.e[mid].chunk0 <= c) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
+// Programmatic dependent launch: wait until the kernels this one depends on have completed; let
+// the next kernel be set up on free resources.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int type) {
   if (type == PARALIA_F32) return static_cast<const float*>(p)[i];
@@ -71,7 +68,8 @@ __device__ __forceinline__ Raw<F32> load_raw(const void* p, int64_t i) {
     r.a = q[0];
     r.b = q[1];
   } else {
-    r.a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+    r.a = q[0];
   }
   return r;
 }
@@ -135,55 +133,75 @@ __device__ __forceinline__ double block_total(double v, double* warp_sums) {
   return s;
 }
 
-// The part of a tensor that chunk c covers: elements [lo, hi), whose groups of eight start at
-// `vec` (lo, or lo + head in the tensor's first chunk).
+// Units [u0, u1) of the launch within tensor e: elements [lo, hi), whose groups of eight start at
+// `vec` (lo, or behind the head at the tensor's beginning).
 struct Span {
   int64_t lo, vec, hi;
 };
-__device__ __forceinline__ Span chunk_span(const GradEntry& e, int c, int chunk) {
+__device__ __forceinline__ Span unit_span(const GradEntry& e, int u0, int u1) {
   Span s;
-  const int64_t first = e.head + (int64_t)(c - e.chunk0) * chunk;
-  s.lo = c == e.chunk0 ? 0 : first;
-  s.vec = first < e.n ? first : e.n;
-  s.hi = min(e.n, first + chunk);
+  const int64_t first = e.head + (int64_t)(u0 - e.unit0) * GL_UNIT;
+  s.lo = u0 == e.unit0 ? 0 : min(first, e.n);
+  s.vec = min(first, e.n);
+  s.hi = min(e.n, e.head + (int64_t)(u1 - e.unit0) * GL_UNIT);
   return s;
 }
 
+// This block's run of units.
+template <int CAP>
+__device__ __forceinline__ int2 block_units(const GradTable<CAP>& t) {
+  return make_int2((int)((int64_t)t.units * blockIdx.x / gridDim.x), (int)((int64_t)t.units * (blockIdx.x + 1) / gridDim.x));
+}
+template <int CAP>
+__device__ __forceinline__ int tensor_end(const GradTable<CAP>& t, int i) {
+  return i + 1 < t.count ? t.e[i + 1].unit0 : t.units;
+}
+
+// The one element outside the groups of eight that this thread has, if any: the first threads take
+// those in front, the threads from 32 on those behind (seven at most each). -1: none.
+__device__ __forceinline__ int64_t odd_element(const Span& s, int64_t groups) {
+  const int t = threadIdx.x;
+  if (t < s.vec - s.lo) return s.lo + t;
+  const int64_t i = s.vec + groups * 8 + t - 32;
+  return t >= 32 && i < s.hi ? i : -1;
+}
+
 template <bool F32>
-__device__ __forceinline__ double chunk_sumsq(const GradEntry& e, const Span& s) {
+__device__ __forceinline__ double span_sumsq(const GradEntry& e, const Span& s) {
   constexpr int U = F32 ? 2 : 4;
   const bool bf = e.src_type == PARALIA_BF16;
   double acc = 0.0;
-  const int64_t groups = (e.flags & GL_SRC_VEC) ? (s.hi - s.vec) / 8 : 0;
-  int64_t g = threadIdx.x;
-  for (; g + (U - 1) * GL_THREADS < groups; g += U * GL_THREADS) {
+  const int64_t groups = (s.hi - s.vec) / 8;
+  const int64_t odd = odd_element(s, groups);
+  const double x = odd >= 0 ? (double)load_any(e.src, odd, e.src_type) : 0.0;   // in flight with the first groups
+  for (int64_t g = threadIdx.x; g < groups; g += U * GL_THREADS) {
     Raw<F32> r[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = load_raw<F32>(e.src, s.vec + (g + u * GL_THREADS) * 8);
+    for (int u = 0; u < U; ++u) {
+      r[u] = Raw<F32>{};
+      if (g + u * GL_THREADS < groups) r[u] = load_raw<F32>(e.src, s.vec + (g + u * GL_THREADS) * 8);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) acc += group_sumsq<F32>(r[u], bf);
   }
-  for (; g < groups; g += GL_THREADS) acc += group_sumsq<F32>(load_raw<F32>(e.src, s.vec + g * 8), bf);
-  for (int64_t i = s.lo + threadIdx.x; i < s.vec; i += GL_THREADS) {
-    const double v = load_any(e.src, i, e.src_type);
-    acc = fma(v, v, acc);
-  }
-  for (int64_t i = s.vec + groups * 8 + threadIdx.x; i < s.hi; i += GL_THREADS) {
-    const double v = load_any(e.src, i, e.src_type);
-    acc = fma(v, v, acc);
-  }
-  return acc;
+  return fma(x, x, acc);
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(GL_THREADS)
+__global__ void __launch_bounds__(GL_THREADS, 3)
 grad_sumsq_kernel(const __grid_constant__ GradTable<CAP> t, double* __restrict__ partials) {
   __shared__ double warp_sums[GL_THREADS / 32];
+  const int2 run = block_units(t);
   double acc = 0.0;
-  for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-    const GradEntry& e = t.e[find_tensor(t, c)];
-    const Span s = chunk_span(e, c, t.chunk);
-    acc += e.src_type == PARALIA_F32 ? chunk_sumsq<true>(e, s) : chunk_sumsq<false>(e, s);
+  int i = t.first[blockIdx.x];
+  pdl_wait();
+  pdl_launch();
+  for (int u = run.x; u < run.y; ++i) {
+    const GradEntry& e = t.e[i];
+    const int end = min(run.y, tensor_end(t, i));
+    const Span s = unit_span(e, u, end);
+    acc += e.src_type == PARALIA_F32 ? span_sumsq<true>(e, s) : span_sumsq<false>(e, s);
+    u = end;
   }
   const double total = block_total(acc, warp_sums);
   if (threadIdx.x == 0) partials[blockIdx.x] = total;
@@ -196,8 +214,10 @@ __device__ __forceinline__ double sum_partials(const double* partials, int used,
 }
 
 __global__ void __launch_bounds__(GL_THREADS)
-grad_norm_final_kernel(const double* __restrict__ partials, int used, double* sumsq, float* norm) {
+grad_norm_final_kernel(const double* partials, int used, double* sumsq, float* norm) {
   __shared__ double warp_sums[GL_THREADS / 32];
+  pdl_wait();
+  pdl_launch();
   const double s = sum_partials(partials, used, warp_sums);
   if (threadIdx.x == 0) {
     if (sumsq) *sumsq = s;
@@ -205,52 +225,94 @@ grad_norm_final_kernel(const double* __restrict__ partials, int used, double* su
   }
 }
 
-template <bool F32>
-__device__ __forceinline__ void chunk_scale(const GradEntry& e, const Span& s, float k0, float k) {
+// Groups of eight from element `from` on: SRC and DST are PARALIA_* types, both sides on 16-byte
+// boundaries.
+template <int SRC, int DST>
+__device__ __forceinline__ void scale_groups(const void* src, void* dst, int64_t from, int groups, float k0, float k) {
+  constexpr bool F32 = SRC == PARALIA_F32;
   constexpr int U = F32 ? 2 : 4;
-  const bool bf = e.src_type == PARALIA_BF16, dbf = e.dst_type == PARALIA_BF16;
-  const int64_t groups = (e.flags & GL_SRC_VEC) ? (s.hi - s.vec) / 8 : 0;
-  auto put = [&](int64_t i, const Raw<F32>& r) {
-    float v[8];
-    to_floats<F32>(r, bf, v);
+  if ((int)threadIdx.x >= groups) return;
+  Raw<F32> r[U];
+  auto fetch = [&](int g) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * k0 * k;
-    if (!(e.flags & GL_DST_VEC)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) store_any(e.dst, i + j, v[j], e.dst_type);
-    } else if (e.dst_type == PARALIA_F32) {
-      float4* q = reinterpret_cast<float4*>(static_cast<float*>(e.dst) + i);
-      q[0] = make_float4(v[0], v[1], v[2], v[3]);
-      q[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(e.dst) + i) =
-          make_uint4(pack16(v[0], v[1], dbf), pack16(v[2], v[3], dbf), pack16(v[4], v[5], dbf),
-                     pack16(v[6], v[7], dbf));
-    }
+    for (int u = 0; u < U; ++u)   // past the end the last group again
+      r[u] = load_raw<F32>(src, from + (int64_t)min(g + u * GL_THREADS, groups - 1) * 8);
   };
-  int64_t g = threadIdx.x;
-  for (; g + (U - 1) * GL_THREADS < groups; g += U * GL_THREADS) {
-    Raw<F32> r[U];
+  for (int g = threadIdx.x; g < groups; g += U * GL_THREADS) {
+    fetch(g);
 #pragma unroll
-    for (int u = 0; u < U; ++u) r[u] = load_raw<F32>(e.src, s.vec + (g + u * GL_THREADS) * 8);
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = from + (int64_t)(g + u * GL_THREADS) * 8;
+      float v[8];
+      to_floats<F32>(r[u], SRC == PARALIA_BF16, v);
 #pragma unroll
-    for (int u = 0; u < U; ++u) put(s.vec + (g + u * GL_THREADS) * 8, r[u]);
+      for (int j = 0; j < 8; ++j) v[j] = v[j] * k0 * k;
+      if (g + u * GL_THREADS < groups) {
+        if constexpr (DST == PARALIA_F32) {
+          float4* q = reinterpret_cast<float4*>(static_cast<float*>(dst) + i);
+          q[0] = make_float4(v[0], v[1], v[2], v[3]);
+          q[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          constexpr bool bf = DST == PARALIA_BF16;
+          *reinterpret_cast<uint4*>(static_cast<uint16_t*>(dst) + i) =
+              make_uint4(pack16(v[0], v[1], bf), pack16(v[2], v[3], bf), pack16(v[4], v[5], bf), pack16(v[6], v[7], bf));
+        }
+      }
+    }
   }
-  for (; g < groups; g += GL_THREADS) put(s.vec + g * 8, load_raw<F32>(e.src, s.vec + g * 8));
-  for (int64_t i = s.lo + threadIdx.x; i < s.vec; i += GL_THREADS)
-    store_any(e.dst, i, load_any(e.src, i, e.src_type) * k0 * k, e.dst_type);
-  for (int64_t i = s.vec + groups * 8 + threadIdx.x; i < s.hi; i += GL_THREADS)
-    store_any(e.dst, i, load_any(e.src, i, e.src_type) * k0 * k, e.dst_type);
+}
+template <int SRC>
+__device__ __forceinline__ void scale_groups_to(int dst_type, const void* src, void* dst, int64_t from, int groups,
+                                                float k0, float k) {
+  if (dst_type == PARALIA_F32) scale_groups<SRC, PARALIA_F32>(src, dst, from, groups, k0, k);
+  else if (dst_type == PARALIA_F16) scale_groups<SRC, PARALIA_F16>(src, dst, from, groups, k0, k);
+  else scale_groups<SRC, PARALIA_BF16>(src, dst, from, groups, k0, k);
 }
 
-// Chunks are taken from the end of the list: what the norm kernel read last is what L2 still
-// holds.
-template <int CAP>
-__global__ void __launch_bounds__(GL_THREADS)
-grad_scale_kernel(const __grid_constant__ GradTable<CAP> t, const double* __restrict__ partials, int used,
+// SRC, DST: the types of every tensor of the list, or -1 where they differ.
+template <int SRC, int DST>
+__device__ __forceinline__ void span_scale(const GradEntry& e, const Span& s, float k0, float k) {
+  const int src_type = SRC >= 0 ? SRC : e.src_type, dst_type = SRC >= 0 ? DST : e.dst_type;
+  if (!(e.flags & GL_DST_VEC)) {
+    // source and destination are out of step: an element at a time, both sides coalesced
+    constexpr int U = 4;
+    for (int64_t i = s.lo + threadIdx.x; i < s.hi; i += U * GL_THREADS) {
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = load_any(e.src, min(i + u * GL_THREADS, s.hi - 1), src_type);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u * GL_THREADS < s.hi) store_any(e.dst, i + u * GL_THREADS, x[u] * k0 * k, dst_type);
+    }
+    return;
+  }
+  const int groups = (int)((s.hi - s.vec) / 8);   // a chunk's at most
+  const int64_t odd = odd_element(s, groups);
+  const float x = odd >= 0 ? load_any(e.src, odd, src_type) : 0.0f;
+  if constexpr (SRC >= 0) scale_groups<SRC, DST>(e.src, e.dst, s.vec, groups, k0, k);
+  else if (src_type == PARALIA_F32) scale_groups_to<PARALIA_F32>(dst_type, e.src, e.dst, s.vec, groups, k0, k);
+  else if (src_type == PARALIA_F16) scale_groups_to<PARALIA_F16>(dst_type, e.src, e.dst, s.vec, groups, k0, k);
+  else scale_groups_to<PARALIA_BF16>(dst_type, e.src, e.dst, s.vec, groups, k0, k);
+  if (odd >= 0) store_any(e.dst, odd, x * k0 * k, dst_type);
+}
+
+// A block takes `chunk` units, the last blocks of the list first: what the norm kernel read last is what
+// L2 still holds. As many blocks as there are chunks, not one for every place on the SMs: 1.4 GB of BF16
+// to as much took 400 us, 473 with blocks that stay and take chunk after chunk (they fall into step,
+// all reading, then all writing).
+template <int CAP, int SRC, int DST>
+__global__ void __launch_bounds__(GL_THREADS, 3)
+grad_scale_kernel(const __grid_constant__ GradTable<CAP> t, const double* __restrict__ partials, int used, int chunk,
                   float max_norm, double* sumsq, float* norm) {
   __shared__ double warp_sums[GL_THREADS / 32];
-  const double total = sum_partials(partials, used, warp_sums);
+  const int u0 = (int)(gridDim.x - 1 - blockIdx.x) * chunk;
+  int u = min(t.units, u0 + chunk);
+  // the tensor with the last unit of the chunk: from the table of starts, a step or two further
+  int i = t.first[(int64_t)(u - 1) * t.starts / t.units];
+  while (i + 1 < t.count && t.e[i + 1].unit0 < u) ++i;
+  pdl_wait();
+  pdl_launch();
+  const double total = used == 1 ? *partials : sum_partials(partials, used, warp_sums);
   const double len = sqrt(total);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (sumsq) *sumsq = total;
@@ -263,12 +325,14 @@ grad_scale_kernel(const __grid_constant__ GradTable<CAP> t, const double* __rest
   const float k0 = factor < 0x1p-90 ? 0x1p-64f : 1.0f;
   if (k0 != 1.0f) factor *= 0x1p64;
   const float k = (float)factor;
-  for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const GradEntry& e = t.e[find_tensor(t, c)];
-    if (k == 1.0f && k0 == 1.0f && (e.flags & GL_IN_PLACE)) continue;
-    const Span s = chunk_span(e, c, t.chunk);
-    if (e.src_type == PARALIA_F32) chunk_scale<true>(e, s, k0, k);
-    else chunk_scale<false>(e, s, k0, k);
+  const bool nothing = k == 1.0f && k0 == 1.0f;
+  while (true) {
+    const GradEntry& e = t.e[i];
+    const int begin = max(u0, e.unit0);
+    if (!(nothing && (e.flags & GL_IN_PLACE))) span_scale<SRC, DST>(e, unit_span(e, begin, u), k0, k);
+    u = begin;
+    if (u <= u0) break;
+    --i;
   }
 }
 
@@ -279,16 +343,20 @@ cudaError_t for_tables(const GradList& l, bool last_first, F f) {
   for (int r = 0; r < runs; ++r) {
     const int i0 = (last_first ? runs - 1 - r : r) * GL_MAX_TENSORS;
     const int n = std::min(GL_MAX_TENSORS, l.count - i0);
-    const int64_t begin = l.entries[i0].chunk0;
-    const int64_t end = i0 + n < l.count ? l.entries[i0 + n].chunk0 : l.chunks;
+    const int64_t begin = l.entries[i0].unit0;
+    const int64_t end = i0 + n < l.count ? l.entries[i0 + n].unit0 : l.units;
     auto fill = [&](auto& t) {
       t.count = n;
-      t.chunk = l.chunk;
-      t.chunk_begin = (int32_t)begin;
-      t.chunks = (int32_t)(end - begin);
+      t.units = (int32_t)(end - begin);
       for (int i = 0; i < n; ++i) {
         t.e[i] = l.entries[i0 + i];
-        t.e[i].chunk0 -= (int32_t)begin;
+        t.e[i].unit0 -= (int32_t)begin;
+      }
+      t.starts = std::min(t.units, GL_NORM_BLOCKS);
+      for (int b = 0, i = 0; b < t.starts; ++b) {
+        const int64_t unit = ((int64_t)t.units * b) / t.starts;
+        while (i + 1 < n && t.e[i + 1].unit0 <= unit) ++i;
+        t.first[b] = (uint16_t)i;
       }
       return f(t);
     };
@@ -310,42 +378,85 @@ cudaError_t for_tables(const GradList& l, bool last_first, F f) {
 
 }  // namespace
 
-int grad_chunk_elements(int64_t total) {
-  // about four chunks for every block of a full grid, between two and eight groups of eight
-  // elements for every thread of a block
-  const int64_t want = total / (GL_MAX_BLOCKS * 4);
-  int chunk = GL_THREADS * 8;
-  while (chunk < want && chunk < GL_THREADS * 64) chunk *= 2;
-  return chunk;
-}
-
 int64_t grad_partials(int64_t count) {
   const int64_t runs = (count + GL_MAX_TENSORS - 1) / GL_MAX_TENSORS;
-  return std::max<int64_t>(1, runs) * GL_MAX_BLOCKS;
+  return std::max<int64_t>(1, runs) * GL_NORM_BLOCKS;
 }
+
+namespace {
+
+template <typename... P, typename... Q>
+cudaError_t launch_after(void (*kernel)(P...), int grid, cudaStream_t stream, Q&&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(GL_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Q>(args)...);
+}
+
+template <int CAP>
+cudaError_t launch_sumsq(const GradTable<CAP>& t, double* partials, int* grid, cudaStream_t stream) {
+  *grid = t.starts;
+  return launch_after(grad_sumsq_kernel<CAP>, t.starts, stream, t, partials);
+}
+template <int CAP>
+cudaError_t launch_scale(const GradTable<CAP>& t, const double* partials, int used, float max_norm, double* sumsq,
+                         float* norm, cudaStream_t stream) {
+  // at most what a block loads at once; a short list is spread over the SMs
+  const int chunk = std::max(1, std::min(GL_CHUNK, t.units / GL_NORM_BLOCKS));
+  const int grid = (t.units + chunk - 1) / chunk;
+  // one pair of types for the whole list, as most lists have it, gets a kernel of its own: a third
+  // fewer registers than the one that looks at every tensor's
+  const int src = t.e[0].src_type, dst = t.e[0].dst_type;
+  bool same = true;
+  for (int i = 1; i < t.count && same; ++i) same = t.e[i].src_type == src && t.e[i].dst_type == dst;
+#define GL_CASE(S, D)                                                                                             \
+  if (same && src == S && dst == D)                                                                               \
+    return launch_after(grad_scale_kernel<CAP, S, D>, grid, stream, t, partials, used, chunk, max_norm, sumsq, norm);
+  GL_CASE(PARALIA_F32, PARALIA_F32)
+  GL_CASE(PARALIA_F32, PARALIA_F16)
+  GL_CASE(PARALIA_F32, PARALIA_BF16)
+  GL_CASE(PARALIA_F16, PARALIA_F32)
+  GL_CASE(PARALIA_F16, PARALIA_F16)
+  GL_CASE(PARALIA_BF16, PARALIA_F32)
+  GL_CASE(PARALIA_BF16, PARALIA_BF16)
+#undef GL_CASE
+  return launch_after(grad_scale_kernel<CAP, -1, -1>, grid, stream, t, partials, used, chunk, max_norm, sumsq, norm);
+}
+
+}  // namespace
 
 cudaError_t launch_grad_sumsq(const GradList& l, double* partials, int* used, cudaStream_t stream) {
   *used = 0;
-  return for_tables(l, false, [&](const auto& t) {
-    const int grid = std::min(t.chunks, GL_MAX_BLOCKS);
-    grad_sumsq_kernel<<<grid, GL_THREADS, 0, stream>>>(t, partials + *used);
+  return for_tables(l, false, [&](auto& t) {
+    int grid = 0;
+    const cudaError_t e = launch_sumsq(t, partials + *used, &grid, stream);
     *used += grid;
-    return cudaGetLastError();
+    return e;
   });
 }
 
 cudaError_t launch_grad_norm_final(const double* partials, int used, double* sumsq, float* norm, cudaStream_t stream) {
-  grad_norm_final_kernel<<<1, GL_THREADS, 0, stream>>>(partials, used, sumsq, norm);
-  return cudaGetLastError();
+  return launch_after(grad_norm_final_kernel, 1, stream, partials, used, sumsq, norm);
 }
 
-cudaError_t launch_grad_scale(const GradList& l, const double* partials, int used, float max_norm, double* sumsq,
+cudaError_t launch_grad_scale(const GradList& l, double* partials, int used, float max_norm, double* sumsq,
                               float* norm, cudaStream_t stream) {
   if (l.count == 0) return launch_grad_norm_final(partials, used, sumsq, norm, stream);
-  return for_tables(l, true, [&](const auto& t) {
-    const int grid = std::min(t.chunks, GL_MAX_BLOCKS);
-    grad_scale_kernel<<<grid, GL_THREADS, 0, stream>>>(t, partials, used, max_norm, sumsq, norm);
-    return cudaGetLastError();
+  if (used > 1 && l.units > (int64_t)GL_CHUNK * GL_NORM_BLOCKS * 2) {
+    // many blocks: the partial sums are added up once and not in each of them
+    const cudaError_t e = launch_grad_norm_final(partials, used, partials, norm, stream);
+    if (e != cudaSuccess) return e;
+    used = 1;
+  }
+  return for_tables(l, true, [&](auto& t) {
+    return launch_scale(t, partials, used, max_norm, sumsq, norm, stream);
   });
 }
 

@@ -5,36 +5,34 @@
 
 namespace paralia {
 
-// Blocks of a launch at most: four of 512 threads for each of 148 SMs.
-constexpr int GL_MAX_BLOCKS = 148 * 4;
+// Blocks of the norm kernel at most: three of 512 threads for each of 148 SMs.
+constexpr int GL_NORM_BLOCKS = 148 * 3;
 // Tensors whose description fits into the parameters of one launch. A longer list takes more.
-constexpr int GL_MAX_TENSORS = 1000;
+constexpr int GL_MAX_TENSORS = 960;
+// Elements of a unit, the grain in which a list is dealt out to the blocks.
+constexpr int GL_UNIT = 2048;
 
-// One tensor of a launch. A chunk is a run of `chunk` elements (GradTable); the first chunk of
-// a tensor also holds the `head` elements in front of the first 16-byte boundary.
+// One tensor of a launch. Its first unit also holds the `head` elements in front of the first
+// 16-byte boundary.
 struct GradEntry {
   const void* src;
   void* dst;
   int64_t n;
-  int32_t chunk0;     // index of the tensor's first chunk in the launch
+  int32_t unit0;      // number of the tensor's first unit in the list
   uint8_t src_type;   // PARALIA_F32 / F16 / BF16
   uint8_t dst_type;
   uint8_t head;
   uint8_t flags;      // GL_*
 };
-constexpr uint8_t GL_SRC_VEC = 1;    // groups of eight can be loaded as 16-byte accesses
-constexpr uint8_t GL_DST_VEC = 2;    // and stored
-constexpr uint8_t GL_IN_PLACE = 4;   // dst is src, of the same type
+constexpr uint8_t GL_DST_VEC = 1;    // groups of eight lie on 16-byte boundaries in dst too
+constexpr uint8_t GL_IN_PLACE = 2;   // dst is src, of the same type
 
 struct GradList {
   int count;                 // tensors with elements
-  GradEntry* entries;        // chunk0 counts over the whole list
-  int64_t chunks;
-  int chunk;                 // elements
+  GradEntry* entries;        // unit0 counts over the whole list
+  int64_t units;
 };
 
-// Elements of a chunk for a list of `total` elements.
-int grad_chunk_elements(int64_t total);
 // Number of partial sums the norm of a list of `count` tensors may leave at most.
 int64_t grad_partials(int64_t count);
 
@@ -43,8 +41,8 @@ cudaError_t launch_grad_sumsq(const GradList& l, double* partials, int* used, cu
 // *sumsq <- sum of the partials, *norm <- its square root (either may be null).
 cudaError_t launch_grad_norm_final(const double* partials, int used, double* sumsq, float* norm, cudaStream_t stream);
 // dst <- src * (norm > max_norm ? max_norm / norm : 1), norm^2 = sum of the `used` partials;
-// writes *sumsq and *norm too (either may be null).
-cudaError_t launch_grad_scale(const GradList& l, const double* partials, int used, float max_norm, double* sumsq,
+// writes *sumsq and *norm too (either may be null). May put the sum in partials[0] if used > 1.
+cudaError_t launch_grad_scale(const GradList& l, double* partials, int used, float max_norm, double* sumsq,
                               float* norm, cudaStream_t stream);
 
 }  // namespace paralia

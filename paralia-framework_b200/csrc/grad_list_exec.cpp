@@ -39,7 +39,6 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
   if (count < 0) return fail(PARALIA_ERR_INVALID_ARG, "negative number of tensors");
   if (count > 0 && (!g || !n || !type)) return fail(PARALIA_ERR_INVALID_ARG, "NULL tensor list");
   if (out && !out_type) return fail(PARALIA_ERR_INVALID_ARG, "outputs without their element types");
-  int64_t total = 0;
   for (int i = 0; i < count; ++i) {
     const int32_t dt = out ? out_type[i] : type[i];
     if (!type_bytes(type[i]) || !type_bytes(dt))
@@ -50,10 +49,8 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
     if (!g[i] || !d) return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: NULL pointer", i);
     if (reinterpret_cast<uintptr_t>(g[i]) % type_bytes(type[i]) || reinterpret_cast<uintptr_t>(d) % type_bytes(dt))
       return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: address is not a multiple of the element size", i);
-    total += n[i];
   }
-  l->chunk = grad_chunk_elements(total);
-  l->chunks = 0;
+  l->units = 0;
   entries->reserve(count);
   std::vector<Range> reads_writes;
   if (writes) reads_writes.reserve(2 * (size_t)count);
@@ -70,19 +67,18 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
     const uintptr_t s = reinterpret_cast<uintptr_t>(e.src), d = reinterpret_cast<uintptr_t>(e.dst);
     const int64_t sb = type_bytes(e.src_type), db = type_bytes(e.dst_type);
     if (e.dst == e.src && e.dst_type == e.src_type) e.flags |= GL_IN_PLACE;
-    // the first element from which loads of eight are aligned, and stores too if that can be
-    for (int h = 7; h >= 0; --h)
-      if (((s + h * sb) & 15) == 0) {
-        const uint8_t both = GL_SRC_VEC | (((d + h * db) & 15) == 0 ? GL_DST_VEC : 0);
-        if (both >= (e.flags & (GL_SRC_VEC | GL_DST_VEC))) {
-          e.flags = (uint8_t)((e.flags & GL_IN_PLACE) | both);
-          e.head = (uint8_t)h;
-        }
-      }
+    // the first element from which groups of eight are aligned, and in dst too if that can be
+    for (int h = 7; h >= 0; --h) {
+      if (((s + h * sb) & 15) != 0) continue;
+      const bool both = ((d + h * db) & 15) == 0;
+      if (!both && (e.flags & GL_DST_VEC)) continue;
+      e.head = (uint8_t)h;
+      if (both) e.flags |= GL_DST_VEC;
+    }
     const int64_t body = std::max<int64_t>(0, e.n - e.head);
-    if (l->chunks > INT32_MAX - body / l->chunk - 1) return fail(PARALIA_ERR_UNSUPPORTED, "the list has too many elements");
-    e.chunk0 = (int32_t)l->chunks;
-    l->chunks += std::max<int64_t>(1, (body + l->chunk - 1) / l->chunk);
+    if (l->units > INT32_MAX - body / GL_UNIT - 1) return fail(PARALIA_ERR_UNSUPPORTED, "the list has too many elements");
+    e.unit0 = (int32_t)l->units;
+    l->units += std::max<int64_t>(1, (body + GL_UNIT - 1) / GL_UNIT);
     entries->push_back(e);
     if (writes) {
       if (!(e.flags & GL_IN_PLACE)) reads_writes.push_back({s, s + (uintptr_t)(e.n * sb), false});
@@ -164,7 +160,8 @@ int exec_tile_grad_scale(int dev, void* stream, int count, const void* const* g,
   if (!sumsq) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq");
   DeviceGuard guard;
   PL_TRY(enter(dev));
-  PL_CUDA(launch_grad_scale(l, sumsq, 1, max_norm, nullptr, norm, static_cast<cudaStream_t>(stream)));
+  // one partial sum is only read
+  PL_CUDA(launch_grad_scale(l, const_cast<double*>(sumsq), 1, max_norm, nullptr, norm, static_cast<cudaStream_t>(stream)));
   return PARALIA_OK;
 }
 
