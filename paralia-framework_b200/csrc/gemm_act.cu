@@ -50,33 +50,49 @@ namespace {
 constexpr int GA_BK = 64;              // k per stage: 128 bytes, one swizzle row
 constexpr int GA_MAX_STAGES = 12;
 constexpr int GA_X_BYTES = 128 * GA_BK * 2;
-constexpr int GA_SMEM = 224 * 1024;    // operand ring and staging buffers
+constexpr int GA_SMEM = 224 * 1024;       // operand ring and staging buffers
+constexpr int GA_SMEM_HALF = 108 * 1024;  // the same where two CTAs share an SM (BN = 64)
 
 // How an operand lies in memory and comes: k contiguous; r / q contiguous, one box for 64 of
 // them; r / q contiguous and a multiple of 64 of them, one box for all of a tile (the tensor map
 // then has the blocks of 64 as a dimension of its own).
 enum : int { GA_K_MAJOR = 0, GA_MN_BOXES = 1, GA_MN_BLOCKS = 2 };
 
-struct GemmActKernelArgs {
+// One product of a launch.
+struct GaProb {
   const void* bias;
   const void* C;
   void* D;
   void* pre;
   int64_t ldC, ldD, ldPre;
-  int32_t tiles;
+  int32_t tile0;                 // number of its first tile in the launch
   int32_t M, N;
   int32_t r_tiles, q_tiles;
   int32_t panel;                 // q tiles per panel of the tile numbering
   int32_t kblocks;
+  int32_t x_mn, y_mn;            // GA_K_MAJOR, GA_MN_BOXES or GA_MN_BLOCKS
+  int32_t tx_bytes;              // what a CTA loads for a stage
+  int32_t act, bf16;
+  int32_t vec;                   // D, C, pre and bias allow 16-byte accesses along M
+  float alpha, beta;
+};
+
+// A launch runs one product or two that do not depend on each other: the two of a gradient are then
+// one wave of tiles, and one launch.
+constexpr int GA_MAX_PROBS = 2;
+struct GaArgs {
+  GaProb p[GA_MAX_PROBS];
+  int32_t tiles;                 // of all products
+  int32_t tiles0;                // of the first
   int32_t bn;                    // columns of a tile: BN, or for BN = 64 any multiple of 16 up to it
   int32_t stages, stage_bytes;   // per CTA
   int32_t split;                 // CTAs that share a tile's k (the cluster, CG == 1)
-  int32_t x_mn, y_mn;            // GA_K_MAJOR, GA_MN_BOXES or GA_MN_BLOCKS
-  int32_t act, bf16;
-  int32_t vec;                   // D, C, pre and bias allow 16-byte accesses along M
-  int32_t stage_out;             // results leave through shared memory by TMA (QC, no split)
-  float alpha, beta;
+  int32_t stage_out;             // results leave through shared memory by TMA (QC, no split),
+  int32_t out_bytes;             // this much of it for each epilogue warp
   int* status;
+};
+struct alignas(64) GaMaps {
+  CUtensorMap x[GA_MAX_PROBS], y[GA_MAX_PROBS], d[GA_MAX_PROBS], pre;
 };
 
 template <int BN>
@@ -243,10 +259,23 @@ __device__ __forceinline__ void ga_tmem_wait16(uint32_t (&r)[16]) {
                : "memory");
 }
 
+__device__ __forceinline__ void ga_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void ga_tmem_wait8(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
 // ------------------------------------------------------------------ epilogue
 // Eight neighbouring rows of one column of D. First Z from sums and bias, then D and Z packed.
 template <bool bf>
-__device__ __forceinline__ void ga_z8(const GemmActKernelArgs& a, const float* v, const uint4& b, float* z) {
+__device__ __forceinline__ void ga_z8(const GaProb& a, const float* v, const uint4& b, float* z) {
   const uint32_t bv[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -256,7 +285,7 @@ __device__ __forceinline__ void ga_z8(const GemmActKernelArgs& a, const float* v
   }
 }
 template <int ACT, bool bf>
-__device__ __forceinline__ void ga_d8(const GemmActKernelArgs& a, const float* z, const uint4& c, uint32_t (&d)[4]) {
+__device__ __forceinline__ void ga_d8(const GaProb& a, const float* z, const uint4& c, uint32_t (&d)[4]) {
   const uint32_t cv[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -286,18 +315,18 @@ __device__ __forceinline__ uint4 ga_load8(const void* p, int64_t valid) {   // o
   if (valid >= 8) return *static_cast<const uint4*>(p);
   return ga_load_any8(static_cast<const uint16_t*>(p), valid);
 }
-__device__ __forceinline__ uint4 ga_load_bias8(const GemmActKernelArgs& a, int64_t m) {
+__device__ __forceinline__ uint4 ga_load_bias8(const GaProb& a, int64_t m) {
   if (!a.bias || m >= a.M) return make_uint4(0, 0, 0, 0);
   return ga_load8(static_cast<const uint16_t*>(a.bias) + m, a.M - m);
 }
-__device__ __forceinline__ uint4 ga_load_c8(const GemmActKernelArgs& a, int64_t m, int64_t n) {
+__device__ __forceinline__ uint4 ga_load_c8(const GaProb& a, int64_t m, int64_t n) {
   if (!a.C || m >= a.M) return make_uint4(0, 0, 0, 0);
   return ga_load8(static_cast<const uint16_t*>(a.C) + m + n * a.ldC, a.M - m);
 }
 
 // Rows m .. m+7 of column n of D (QC): acc -> D, pre.
 template <int ACT, bool bf>
-__device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m, int64_t n, float* v) {
+__device__ __forceinline__ void ga_finish8(const GaProb& a, int64_t m, int64_t n, float* v) {
   if (a.vec && m + 8 <= a.M) {
     float zf[8];
     uint32_t z[4], d[4];
@@ -321,7 +350,7 @@ __device__ __forceinline__ void ga_finish8(const GemmActKernelArgs& a, int64_t m
 
 // W accumulator columns q0 .. q0+W-1 of lane row r.
 template <bool QC, int W>
-__device__ __forceinline__ void ga_finish(const GemmActKernelArgs& a, int64_t r, int64_t q0, float (&v)[W]) {
+__device__ __forceinline__ void ga_finish(const GaProb& a, int64_t r, int64_t q0, float (&v)[W]) {
   with_act_type(a.act, a.bf16 != 0, [&](auto t, auto y) {
     constexpr int ACT = decltype(t)::value;
     constexpr bool bf = decltype(y)::value != 0;
@@ -361,7 +390,7 @@ __device__ __forceinline__ void ga_finish(const GemmActKernelArgs& a, int64_t r,
 // is not unrolled: with ten variants and eight warps out of step the instruction cache is what an
 // unrolled one waits for (8192 x 8192 x 1024 with tanh-GELU: 174 us unrolled by four).
 template <int ACT, bool bf>
-__device__ __forceinline__ void ga_staged_tile(const GemmActKernelArgs& a, const CUtensorMap* map_d,
+__device__ __forceinline__ void ga_staged_tile(const GaProb& a, const CUtensorMap* map_d,
                                                const CUtensorMap* map_pre, uint32_t taddr, uint32_t out, int q,
                                                int r_first, int cols, int lane) {
   const uint32_t row = out + lane * 128;
@@ -417,10 +446,59 @@ __device__ __forceinline__ void ga_staged_tile(const GemmActKernelArgs& a, const
   }
 }
 
+// The same for QC == false: row r of D in columns q .. q+cols-1. A warp's access to a column is 64
+// contiguous bytes wherever it starts. C of the next eight columns is fetched with their sums.
+template <int ACT, bool bf>
+__device__ __forceinline__ void ga_direct_tile(const GaProb& a, uint32_t taddr, int64_t r, int64_t q, int cols) {
+  const int last = (int)min((int64_t)cols, a.N - q);
+  if (last <= 0) return;
+  const bool in = r < a.M;
+  const int64_t m = min(r, (int64_t)a.M - 1);
+  const float b = a.bias ? load16(a.bias, m, bf) : 0.0f;
+  const uint16_t* cp = static_cast<const uint16_t*>(a.C) + m + q * a.ldC;
+  uint16_t* dp = static_cast<uint16_t*>(a.D) + m + q * a.ldD;
+  uint16_t* pp = static_cast<uint16_t*>(a.pre) + m + q * a.ldPre;
+  uint32_t v[8], c[8] = {};
+  auto fetch = [&](int at) {
+    ga_tmem_ld8(taddr + at, v);
+    if (a.C) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c[j] = *cp;
+        if (at + j + 1 < last) cp += a.ldC;   // past the last column the last one again
+      }
+    }
+  };
+  fetch(0);
+#pragma unroll 1
+  for (int at = 0; at < last; at += 8) {
+    ga_tmem_wait8(v);
+    float z[8];
+    uint32_t cx[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      z[j] = fmaf(a.alpha, a.kblocks == 0 ? 0.0f : __uint_as_float(v[j]), b);
+      cx[j] = c[j];
+    }
+    if (at + 8 < last) fetch(at + 8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float d = act_value<ACT>(z[j]);
+      if (a.C) d = fmaf(a.beta, unpack16(cx[j], bf).x, d);
+      if (in && at + j < last) {
+        store16(dp, 0, d, bf);
+        if (a.pre) store16(pp, 0, z[j], bf);
+      }
+      dp += a.ldD;
+      pp += a.ldPre;
+    }
+  }
+}
+
 // Asks L2 for the rows m0 .. m0+rows-1 of the bias and of `cols` columns of C from n0 on. The epilogue's
 // own loads come late and few at a time, each with the latency of where the line then is.
 template <int THREADS>
-__device__ __forceinline__ void ga_prefetch_inputs(const GemmActKernelArgs& a, int64_t m0, int rows, int64_t n0, int cols) {
+__device__ __forceinline__ void ga_prefetch_inputs(const GaProb& a, int64_t m0, int rows, int64_t n0, int cols) {
   const int e = threadIdx.x - 64, lines = (rows + 63) / 64;
   if (a.bias && e < lines && m0 + e * 64 < a.M)
     asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint16_t*>(a.bias) + m0 + e * 64));
@@ -438,9 +516,9 @@ struct GaTile {
 };
 // Tiles are numbered in panels of a few q tiles, inside a panel along q first: what runs at
 // one time then shares few X and few Y tiles, which cuts what is pulled through L2.
-__device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int tile) {
+__device__ __forceinline__ GaTile ga_tile(const GaProb& a, int tile) {
   const uint32_t per_panel = (uint32_t)a.r_tiles * (uint32_t)a.panel;
-  const uint32_t panel = (uint32_t)tile / per_panel, rest = (uint32_t)tile - panel * per_panel;
+  const uint32_t number = (uint32_t)(tile - a.tile0), panel = number / per_panel, rest = number - panel * per_panel;
   const uint32_t width = min((uint32_t)a.panel, (uint32_t)a.q_tiles - panel * (uint32_t)a.panel);
   GaTile t;
   t.rt = (int)(rest / width);
@@ -450,9 +528,7 @@ __device__ __forceinline__ GaTile ga_tile(const GemmActKernelArgs& a, int tile) 
 
 template <int BN, int CG, bool QC>
 __global__ void __launch_bounds__(GaShape<BN>::THREADS, BN == 64 ? 2 : 1)
-gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
-                const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_pre,
-                const __grid_constant__ GemmActKernelArgs a) {
+gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaArgs g) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -462,18 +538,18 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   constexpr int EW = GaShape<BN>::EPILOGUE_WARPS;
   constexpr int YROWS = BN / CG;                       // rows of Y this CTA loads
   constexpr uint32_t TMEM_COLS = 2 * BN;
-  const int bn = BN == 64 && !QC ? a.bn : BN;
+  const int bn = BN == 64 && !QC ? g.bn : BN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = (CG == 2 || a.split > 1) ? cluster_rank() : 0;
-  const int split = CG == 1 ? a.split : 1;
+  const uint32_t rank = (CG == 2 || g.split > 1) ? cluster_rank() : 0;
+  const int split = CG == 1 ? g.split : 1;
   const int group = CG * split;                        // CTAs that share a tile
   const int first_tile = blockIdx.x / group, tile_step = gridDim.x / group;
-  // this CTA's run of k blocks
-  const int kb0 = split > 1 ? (int)((int64_t)a.kblocks * rank / split) : 0;
-  const int kb1 = split > 1 ? (int)((int64_t)a.kblocks * (rank + 1) / split) : a.kblocks;
+  // this CTA's run of a product's k blocks
+  auto k_begin = [&](const GaProb& a) { return split > 1 ? (int)((int64_t)a.kblocks * rank / split) : 0; };
+  auto k_end = [&](const GaProb& a) { return split > 1 ? (int)((int64_t)a.kblocks * (rank + 1) / split) : a.kblocks; };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
+    for (int s = 0; s < g.stages; ++s) {
       mbar_init(&ctl->full[s], 1);
       mbar_init(&ctl->empty[s], 1);
     }
@@ -484,8 +560,10 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     ctl->abort_flag = 0;
     ctl->tmem_base = 0;
     mbar_fence_init();
-    prefetch_tensormap(&map_x);
-    prefetch_tensormap(&map_y);
+    if (g.p[0].kblocks > 0) {
+      prefetch_tensormap(&maps.x[0]);
+      prefetch_tensormap(&maps.y[0]);
+    }
   }
   __syncthreads();
   if (warp == 1) {
@@ -517,13 +595,19 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   if (warp == 0) {
     // ------------------------------ producer ------------------------------
     const uint64_t pol_x = ga_policy_stream(), pol_y = ga_policy_normal();
-    // how far one k block moves the first two coordinates of a box
-    const int xk0 = a.x_mn ? 0 : GA_BK, xk1 = a.x_mn ? GA_BK : 0;
-    const int yk0 = a.y_mn ? 0 : GA_BK, yk1 = a.y_mn ? GA_BK : 0;
     int s = 0, filled = 0;           // stage, and how many stages have been filled at all (capped)
     uint32_t phase = 0;              // parity of the ring's round
     bool ok = true;
-    for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step) {
+    for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step) {
+      const int which = tile >= g.tiles0 ? 1 : 0;
+      const GaProb& a = g.p[which];
+      const CUtensorMap *map_x = &maps.x[which], *map_y = &maps.y[which];
+      const int kb0 = k_begin(a), kb1 = k_end(a);
+      // how far one k block moves the first two coordinates of a box
+      const int xk0 = a.x_mn ? 0 : GA_BK, xk1 = a.x_mn ? GA_BK : 0;
+      const int yk0 = a.y_mn ? 0 : GA_BK, yk1 = a.y_mn ? GA_BK : 0;
+      const bool x_boxes = a.x_mn == GA_MN_BOXES, y_boxes = a.y_mn == GA_MN_BOXES;
+      const uint32_t tx = a.tx_bytes * CG;
       const GaTile t = ga_tile(a, tile);
       const int r0 = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0);
       const int q0 = t.qt * bn + (CG == 2 ? (int)rank * YROWS : 0);
@@ -531,27 +615,27 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       int y0 = a.y_mn == GA_MN_BOXES ? q0 : a.y_mn ? 0 : kb0 * GA_BK, y1 = a.y_mn ? kb0 * GA_BK : q0;
       const int x2 = a.x_mn == GA_MN_BLOCKS ? r0 / 64 : 0, y2 = a.y_mn == GA_MN_BLOCKS ? q0 / 64 : 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (filled == a.stages && !warp_wait(&ctl->empty[s], phase ^ 1u, abort_flag)) {
-          if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_EMPTY_WAIT_TIMEOUT); }
+        if (filled == g.stages && !warp_wait(&ctl->empty[s], phase ^ 1u, abort_flag)) {
+          if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_EMPTY_WAIT_TIMEOUT); }
           ok = false;
           break;
         }
         if (elect_one()) {
-          const uint32_t x = smem_u32(smem) + s * a.stage_bytes, y = x + GA_X_BYTES;
+          const uint32_t x = smem_u32(smem) + s * g.stage_bytes, y = x + GA_X_BYTES;
           uint32_t bar = smem_u32(&ctl->full[s]);
           if (CG == 2) bar = map_rank(bar, 0);
-          if (CG == 1 || rank == 0) mbar_expect_tx(&ctl->full[s], a.stage_bytes * CG);
-          ga_load<CG>(x, &map_x, bar, pol_x, x0, x1, x2);
-          if (a.x_mn == GA_MN_BOXES) ga_load<CG>(x + 8192, &map_x, bar, pol_x, x0 + 64, x1, 0);
-          ga_load<CG>(y, &map_y, bar, pol_y, y0, y1, y2);
-          if (a.y_mn == GA_MN_BOXES) {
+          if (CG == 1 || rank == 0) mbar_expect_tx(&ctl->full[s], tx);
+          ga_load<CG>(x, map_x, bar, pol_x, x0, x1, x2);
+          if (x_boxes) ga_load<CG>(x + 8192, map_x, bar, pol_x, x0 + 64, x1, 0);
+          ga_load<CG>(y, map_y, bar, pol_y, y0, y1, y2);
+          if (y_boxes) {
 #pragma unroll
-            for (int j = 1; j < YROWS / 64; ++j) ga_load<CG>(y + j * 8192, &map_y, bar, pol_y, y0 + j * 64, y1, 0);
+            for (int j = 1; j < YROWS / 64; ++j) ga_load<CG>(y + j * 8192, map_y, bar, pol_y, y0 + j * 64, y1, 0);
           }
         }
         x0 += xk0; x1 += xk1; y0 += yk0; y1 += yk1;
-        if (filled < a.stages) ++filled;
-        if (++s == a.stages) { s = 0; phase ^= 1u; }
+        if (filled < g.stages) ++filled;
+        if (++s == g.stages) { s = 0; phase ^= 1u; }
       }
     }
     // Before shared memory is given up: every stage has been read by its MMAs (with CG == 2 the
@@ -560,53 +644,55 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
     for (int j = 0; j < filled; ++j) {
       // the oldest stage first; `s` and `phase` are those of the next fill
       int zero = 0;
-      const int q = filled < a.stages ? j : (s + j < a.stages ? s + j : s + j - a.stages);
-      const uint32_t parity = filled < a.stages || q < s ? phase : phase ^ 1u;
+      const int q = filled < g.stages ? j : (s + j < g.stages ? s + j : s + j - g.stages);
+      const uint32_t parity = filled < g.stages || q < s ? phase : phase ^ 1u;
       const bool clean = __all_sync(0xffffffffu, ok && !*abort_flag);
       if (CG == 2 && rank != 0 && !clean) break;   // its copies signal the leader
       if (!warp_wait(clean ? &ctl->empty[q] : &ctl->full[q], parity, &zero)) {
         *abort_flag = 1;
-        atomicExch(a.status, KERR_DRAIN_TIMEOUT);
+        atomicExch(g.status, KERR_DRAIN_TIMEOUT);
         break;
       }
     }
   } else if (warp == 1) {
     // ------------------------------ MMA issuer ------------------------------
     if (CG == 1 || rank == 0) {
-      const uint32_t fmt = a.bf16 ? 1u : 0u;
-      const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a.x_mn ? 1u << 15 : 0u) | (a.y_mn ? 1u << 16 : 0u) |
-                             ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
-      const uint32_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
-      const uint64_t x_desc = ga_desc(smem_u32(smem), a.x_mn), y_desc = ga_desc(smem_u32(smem) + GA_X_BYTES, a.y_mn);
       int s = 0;
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+      for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step, ++local) {
         const int buf = local & 1;
         if (local >= 2 && !warp_wait(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
-          if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
+          if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_TMEM_WAIT_TIMEOUT); }
           ok = false;
           break;
         }
+        const GaProb& a = g.p[tile >= g.tiles0 ? 1 : 0];
+        const int kb0 = k_begin(a), kb1 = k_end(a);
+        const uint32_t fmt = a.bf16 ? 1u : 0u;
+        const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a.x_mn ? 1u << 15 : 0u) | (a.y_mn ? 1u << 16 : 0u) |
+                               ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+        const uint32_t x_step = a.x_mn ? (2048 >> 4) : (32 >> 4), y_step = a.y_mn ? (2048 >> 4) : (32 >> 4);
+        const uint64_t x_desc = ga_desc(smem_u32(smem), a.x_mn), y_desc = ga_desc(smem_u32(smem) + GA_X_BYTES, a.y_mn);
         ga_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(buf * BN);
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!warp_wait(&ctl->full[s], phase, abort_flag)) {
-            if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_FULL_WAIT_TIMEOUT); }
+            if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_FULL_WAIT_TIMEOUT); }
             ok = false;
             break;
           }
           ga_fence_after();
           if (elect_one()) {
-            const uint64_t dx = x_desc + (uint32_t)(s * (a.stage_bytes >> 4)), dy = y_desc + (uint32_t)(s * (a.stage_bytes >> 4));
+            const uint64_t dx = x_desc + (uint32_t)(s * (g.stage_bytes >> 4)), dy = y_desc + (uint32_t)(s * (g.stage_bytes >> 4));
 #pragma unroll
             for (int j = 0; j < GA_BK / 16; ++j)
               ga_mma<CG>(d, dx + j * x_step, dy + j * y_step, idesc, (kb > kb0 || j > 0) ? 1u : 0u);
             ga_commit<CG>(&ctl->empty[s]);
           }
           __syncwarp();
-          if (++s == a.stages) { s = 0; phase ^= 1u; }
+          if (++s == g.stages) { s = 0; phase ^= 1u; }
         }
         if (ok && elect_one()) ga_commit<CG>(&ctl->acc_full[buf]);
         __syncwarp();
@@ -615,12 +701,13 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
   } else {
     // ------------------------------ epilogue ------------------------------
     const int quad = warp & 3, part = (warp - 2) >> 2;   // lanes of tensor memory; share of the columns
-    constexpr int W = 16;
     const int part_cols = bn / (EW / 4);
     int local = 0;
     bool ok = true;
-    for (int tile = first_tile; tile < a.tiles && ok; tile += tile_step, ++local) {
+    for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step, ++local) {
       const int buf = local & 1;
+      const int which = tile >= g.tiles0 ? 1 : 0;
+      const GaProb& a = g.p[which];
       const GaTile t = ga_tile(a, tile);
       {
         // what the epilogue will read, into L2 while the product runs
@@ -631,7 +718,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
                                     QC ? 128 : q_cols);
       }
       if (!mbar_wait_bounded(&ctl->acc_full[buf], (uint32_t)((local >> 1) & 1), abort_flag)) {
-        if (!*abort_flag) { *abort_flag = 1; atomicExch(a.status, KERR_TMEM_WAIT_TIMEOUT); }
+        if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_TMEM_WAIT_TIMEOUT); }
         ok = false;
         break;
       }
@@ -640,41 +727,30 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       const int64_t q = (int64_t)t.qt * bn + part * part_cols;
       const uint32_t taddr = tmem_base + ((uint32_t)(quad * 32) << 16) + (uint32_t)(buf * BN + part * part_cols);
       if constexpr (QC) {
-        if (a.stage_out) {
-          const uint32_t out = smem_u32(smem) + a.stages * a.stage_bytes + (warp - 2) * (a.pre ? 8192 : 4096);
+        if (g.stage_out) {
+          const uint32_t out = smem_u32(smem) + g.stages * g.stage_bytes + (warp - 2) * g.out_bytes;
           const int r_first = t.rt * (128 * CG) + (CG == 2 ? (int)rank * 128 : 0) + quad * 32;
           with_act_type(a.act, a.bf16 != 0, [&](auto k, auto y) {
-            ga_staged_tile<decltype(k)::value, decltype(y)::value != 0>(a, &map_d, &map_pre, taddr, out, (int)q, r_first,
+            ga_staged_tile<decltype(k)::value, decltype(y)::value != 0>(a, &maps.d[which], &maps.pre, taddr, out, (int)q, r_first,
                                                                         part_cols, lane);
           });
         }
       }
+      if (split > 1) {
 #pragma unroll 1
-      for (int c = 0; c < part_cols && !(QC && a.stage_out); c += W) {
-        uint32_t raw[W];
-        ga_tmem_ld16(taddr + c, raw);
-        ga_tmem_wait16(raw);
-        float v[W];
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = __uint_as_float(raw[j]);
-        if (a.kblocks == 0) {
-#pragma unroll
-          for (int j = 0; j < W; ++j) v[j] = 0.0f;   // the accumulator was never written
-        }
-        if (split > 1) {
+        for (int c = 0; c < part_cols; c += 16) {
+          uint32_t v[16];
+          ga_tmem_ld16(taddr + c, v);
+          ga_tmem_wait16(v);
           // column-major FP32 in the operand ring, which nothing reads any more
           float* stage = reinterpret_cast<float*>(smem) + (part * part_cols + c) * 128 + quad * 32 + lane;
 #pragma unroll
-          for (int j = 0; j < W; ++j) stage[j * 128] = v[j];
-        } else if constexpr (!QC) {
-#pragma unroll 1
-          for (int g = 0; g < W; g += 8) {
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = g == 0 ? v[j] : v[8 + j];
-            ga_finish<QC, 8>(a, r, q + c + g, x);
-          }
+          for (int j = 0; j < 16; ++j) stage[j * 128] = __uint_as_float(v[j]);
         }
+      } else if constexpr (!QC) {
+        with_act_type(a.act, a.bf16 != 0, [&](auto k, auto y) {
+          ga_direct_tile<decltype(k)::value, decltype(y)::value != 0>(a, taddr, r, q, part_cols);
+        });
       }
       ga_fence_before();
       __syncwarp();
@@ -694,6 +770,7 @@ gemm_act_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
       // A warp sums one column of this CTA's share at a time, a lane four rows of it: 512 contiguous
       // bytes from each CTA. The sums replace this CTA's own share, which nobody else reads.
       const int cols = bn / split;                    // columns of this CTA
+      const GaProb& a = g.p[first_tile >= g.tiles0 ? 1 : 0];
       const GaTile t = ga_tile(a, first_tile);
       float* own = reinterpret_cast<float*>(smem) + (int)rank * cols * 128;
       // columns that exist (QC: all, the others are cut off later)
@@ -785,85 +862,117 @@ __global__ void __launch_bounds__(256) align_copy_kernel(const __grid_constant__
 }
 
 // ------------------------------------------------------------------ gradient of the epilogue
-constexpr int AG_ROWS = 256;     // rows of a block: 32 lanes x 8
+constexpr int AG_ROWS = 64;      // rows of a block: eight lanes x 8
 constexpr int AG_WARPS = 8;
+constexpr int AG_COLS = 4 * AG_WARPS;   // columns that a block works on at a time
+constexpr int AG_U = 2;          // columns in flight per thread
 
-// A block takes AG_ROWS rows and a run of columns; a warp walks every AG_WARPS-th column of
-// the run, a lane holds eight rows, so the row sums of the bias gradient stay in registers.
-// The sums of the eight warps meet in shared memory in warp order and leave as one partial
-// per row and run; act_grad_bias_kernel adds the runs in order.
+// The `parts` blocks of a cluster take AG_ROWS rows, each a run of the columns; eight lanes hold a column's
+// rows, eight each, a warp four columns and then every AG_COLS-th one, so the row sums of the bias
+// gradient stay in registers. The sums of the lanes meet by shuffles, those of the warps in shared memory
+// in warp order, those of the blocks through distributed shared memory in rank order: one launch, no
+// scratch, the same bits every time (a second kernel that added up to 99 partial sums a row took 11 us
+// beside 12 of this one).
 //
-// Bound by memory: two reads and one write of two bytes per entry. VEC: rows come and go as
-// 16-byte accesses (eight rows of a lane are neighbours); otherwise a lane's eight rows lie
-// 32 apart and every access is of one element, coalesced over the warp at any alignment.
+// Bound by memory: two reads and one write of two bytes per entry. VEC: rows come and go as 16-byte
+// accesses (eight rows of a lane are neighbours), AG_U columns of a lane in flight; otherwise a lane
+// holds two rows 32 apart and every access is of one element, coalesced over the warp at any alignment.
 template <bool VEC>
-__global__ void __launch_bounds__(AG_WARPS * 32) act_grad_kernel(const ActGradProblem p, int cols) {
+__global__ void __launch_bounds__(AG_WARPS * 32) act_grad_kernel(const __grid_constant__ ActGradProblem p, int parts) {
   __shared__ float sums[AG_WARPS][AG_ROWS];
+  __shared__ float total[AG_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row0 = (int64_t)blockIdx.x * AG_ROWS;
-  const int64_t n_begin = (int64_t)blockIdx.y * cols;
-  const int64_t n_end = min((int64_t)p.N, n_begin + cols);
+  const int part = blockIdx.x % parts;
+  const int64_t row0 = (int64_t)(blockIdx.x / parts) * AG_ROWS;
+  const int n_begin = (int)((int64_t)p.N * part / parts), n_end = (int)((int64_t)p.N * (part + 1) / parts);
   float acc[8] = {};
+  pdl_wait();
+  pdl_launch();
   with_act_type(p.act, p.bf16 != 0, [&](auto a, auto y) {
     constexpr int ACT = decltype(a)::value;
     constexpr bool bf = decltype(y)::value != 0;
-    for (int64_t n = n_begin + warp; n < n_end; n += AG_WARPS) {
-      if (VEC) {
-        const int64_t m = row0 + lane * 8;
-        if (m + 8 <= p.M) {
-          const uint4 d = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.dD) + m + n * p.ldD);
-          uint4 z = make_uint4(0, 0, 0, 0);
-          if (ACT != PARALIA_ACT_NONE)
-            z = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.pre) + m + n * p.ldPre);
-          const uint32_t dv[4] = {d.x, d.y, d.z, d.w}, zv[4] = {z.x, z.y, z.z, z.w};
-          uint32_t o[4];
+    const uint16_t* dd = static_cast<const uint16_t*>(p.dD);
+    const uint16_t* pre = static_cast<const uint16_t*>(p.pre);
+    uint16_t* dz = static_cast<uint16_t*>(p.dZ);
+    // a select for relu, so that an infinite dD in a place that it has closed gives 0
+    auto value = [&](float g, float q) { return ACT == PARALIA_ACT_RELU ? (q > 0.0f ? g : 0.0f) : g * act_slope<ACT>(q); };
+    const int64_t m = row0 + (lane & 7) * 8;
+    const int first = n_begin + warp * 4 + (lane >> 3);
+    if (VEC && m + 8 <= p.M) {
+      auto finish = [&](int n, const uint4& d, const uint4& z) {
+        const uint32_t dv[4] = {d.x, d.y, d.z, d.w}, zv[4] = {z.x, z.y, z.z, z.w};
+        uint32_t o[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 g = unpack16(dv[i], bf), q = unpack16(zv[i], bf);
-            // a select, so that an infinite dD in a place that relu has closed gives 0
-            const float g0 = ACT == PARALIA_ACT_RELU ? (q.x > 0.0f ? g.x : 0.0f) : g.x * act_slope<ACT>(q.x);
-            const float g1 = ACT == PARALIA_ACT_RELU ? (q.y > 0.0f ? g.y : 0.0f) : g.y * act_slope<ACT>(q.y);
-            acc[2 * i] += g0;
-            acc[2 * i + 1] += g1;
-            o[i] = pack16(g0, g1, bf);
-          }
-          if (p.dZ)
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dZ) + m + n * p.ldZ) = make_uint4(o[0], o[1], o[2], o[3]);
-          continue;
+        for (int i = 0; i < 4; ++i) {
+          const float2 g = unpack16(dv[i], bf), q = unpack16(zv[i], bf);
+          const float g0 = value(g.x, q.x), g1 = value(g.y, q.y);
+          acc[2 * i] += g0;
+          acc[2 * i + 1] += g1;
+          o[i] = pack16(g0, g1, bf);
         }
-      }
+        if (dz) *reinterpret_cast<uint4*>(dz + m + n * p.ldZ) = make_uint4(o[0], o[1], o[2], o[3]);
+      };
+      for (int n = first; n < n_end; n += AG_U * AG_COLS) {
+        uint4 d[AG_U], z[AG_U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t m = VEC ? row0 + lane * 8 + i : row0 + lane + 32 * i;
-        if (m >= p.M) continue;
-        const float g = load16(p.dD, m + n * p.ldD, bf);
-        const float q = ACT != PARALIA_ACT_NONE ? load16(p.pre, m + n * p.ldPre, bf) : 0.0f;
-        const float v = ACT == PARALIA_ACT_RELU ? (q > 0.0f ? g : 0.0f) : g * act_slope<ACT>(q);
-        acc[i] += v;
-        if (p.dZ) store16(p.dZ, m + n * p.ldZ, v, bf);
+        for (int u = 0; u < AG_U; ++u) {
+          const int64_t c = min(n + u * AG_COLS, n_end - 1);   // past the end the last column again
+          d[u] = *reinterpret_cast<const uint4*>(dd + m + c * p.ldD);
+          z[u] = ACT != PARALIA_ACT_NONE ? *reinterpret_cast<const uint4*>(pre + m + c * p.ldPre) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < AG_U; ++u)
+          if (n + u * AG_COLS < n_end) finish(n + u * AG_COLS, d[u], z[u]);
+      }
+    } else {
+      for (int n = VEC ? first : n_begin + warp; n < n_end; n += VEC ? AG_COLS : AG_WARPS) {
+#pragma unroll
+        for (int i = 0; i < (VEC ? 8 : 2); ++i) {
+          const int64_t r = VEC ? m + i : row0 + lane + 32 * i;
+          if (r >= p.M) continue;
+          const float v = value(load16(dd, r + n * p.ldD, bf), ACT != PARALIA_ACT_NONE ? load16(pre, r + n * p.ldPre, bf) : 0.0f);
+          acc[i] += v;
+          if (dz) store16(dz, r + n * p.ldZ, v, bf);
+        }
       }
     }
   });
   if (!p.dbias) return;
+  if (VEC) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sums[warp][VEC ? lane * 8 + i : lane + 32 * i] = acc[i];
+    for (int i = 0; i < 8; ++i) {
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
+      acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);
+      if (lane < 8) sums[warp][lane * 8 + i] = acc[i];
+    }
+  } else {
+    sums[warp][lane] = acc[0];
+    sums[warp][lane + 32] = acc[1];
+  }
   __syncthreads();
-  const int64_t m = row0 + threadIdx.x;
-  if (m < p.M) {
+  if (threadIdx.x < AG_ROWS) {
     float s = 0.0f;
 #pragma unroll
     for (int w = 0; w < AG_WARPS; ++w) s += sums[w][threadIdx.x];
-    p.partials[(int64_t)blockIdx.y * p.M + m] = s;
+    total[threadIdx.x] = s;
   }
-}
-
-__global__ void __launch_bounds__(256) act_grad_bias_kernel(const ActGradProblem p, int chunks) {
-  const int64_t m = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (m >= p.M) return;
-  float s = 0.0f;
-  for (int c = 0; c < chunks; ++c) s += p.partials[(int64_t)c * p.M + m];
-  if (p.beta_bias != 0.0f) s = fmaf(p.beta_bias, load16(p.dbias, m, p.bf16 != 0), s);
-  store16(p.dbias, m, s, p.bf16 != 0);
+  if (parts > 1) cluster_sync();
+  else __syncthreads();
+  const int rows = AG_ROWS / parts;      // rows that this block finishes
+  const int64_t row = row0 + part * rows + threadIdx.x;
+  if ((int)threadIdx.x < rows && row < p.M) {
+    const uint32_t at = smem_u32(&total[part * rows + threadIdx.x]);
+    float t = 0.0f;
+    for (int b = 0; b < parts; ++b) {
+      float x;
+      if (parts > 1) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(map_rank(at, b)) : "memory");
+      else x = total[part * rows + threadIdx.x];
+      t += x;
+    }
+    if (p.beta_bias != 0.0f) t = fmaf(p.beta_bias, load16(p.dbias, row, p.bf16 != 0), t);
+    store16(p.dbias, row, t, p.bf16 != 0);
+  }
+  if (parts > 1) cluster_sync();         // nobody leaves while its sums are still read
 }
 
 inline bool vec16(const void* p, int64_t ld) {
@@ -906,14 +1015,27 @@ struct GaPlan {
 
 constexpr int GA_SMS = 148;
 
+int64_t ga_tiles(const GaPlan& v, int64_t M, int64_t N) {
+  const int64_t R = v.qc ? N : M, Q = v.qc ? M : N;
+  return ((R + 128 * v.cg - 1) / (128 * v.cg)) * ((Q + v.bn - 1) / v.bn);
+}
+
 // Estimated microseconds of a variant (a constant common to all is left out). The constants are a fit
 // to 3100 timings of 134 shapes (1 to 2048 columns, 300 to 16384 rows, k 256 to 10240) with every
 // variant that fits them: the variant it picks is 1.2 % slower than the fastest in the mean, 30 % at
 // worst (1024 x 37 x 1024, 6.9 against 5.3 us).
-double ga_cost(const GaPlan& v, int64_t M, int64_t N, int64_t K) {
-  const int64_t R = v.qc ? N : M, Q = v.qc ? M : N;
-  const int64_t tiles = ((R + 128 * v.cg - 1) / (128 * v.cg)) * ((Q + v.bn - 1) / v.bn);
-  const int64_t run = ((K + GA_BK - 1) / GA_BK + v.split - 1) / v.split;   // k blocks of a CTA
+double ga_cost(const GaPlan& v, const GemmActProblem* ps, int count) {
+  int64_t tiles = 0, run = 0;
+  double hbm_bytes = 0.0, runs = 0.0;
+  for (int i = 0; i < count; ++i) {
+    const int64_t t = ga_tiles(v, ps[i].M, ps[i].N);
+    const int64_t r = ((ps[i].K + GA_BK - 1) / GA_BK + v.split - 1) / v.split;   // k blocks of a CTA
+    tiles += t;
+    runs += (double)t * r;
+    run = std::max(run, r);
+    hbm_bytes += 2.0 * ((double)ps[i].M * ps[i].K + (double)ps[i].K * ps[i].N + (double)ps[i].M * ps[i].N);
+  }
+  const double mean_run = runs / tiles;
   const int64_t ctas = tiles * v.cg * v.split;
   const int per_sm = v.bn <= 64 ? 2 : 1;
   // CTAs an SM gets: clusters of 4 and 8 do not fill every group of SMs, 36 and 16 fit at a time
@@ -925,23 +1047,25 @@ double ga_cost(const GaPlan& v, int64_t M, int64_t N, int64_t K) {
   // a k block: MMAs at 1.4 times BN x 2 clocks, its bytes at 130 GB/s an SM, and 0.23 us from a CTA
   // that runs by itself
   const double bytes = (128.0 + (double)v.bn / v.cg) * 128.0;
-  const double sm = (double)run * std::max(share * std::max(v.bn * 2 / 1900.0 * 1.4, bytes / 130e3), turns * 0.23);
+  const double sm = std::max(mean_run * share, (double)run) * std::max(v.bn * 2 / 1900.0 * 1.4, bytes / 130e3);
+  const double alone = std::max(mean_run * turns, (double)run) * 0.23;
   const double in_flight = std::min(1.0, (double)ctas / (2 * GA_SMS));
-  const double hbm = 2.0 * ((double)M * K + (double)K * N + (double)M * N) / 6.6e6 / (0.88 + 0.12 * in_flight);
-  const double l2 = (double)ctas * run * bytes / 15e6;
-  return std::max(sm, std::max(hbm, l2)) + 0.0079 * v.bn / v.split + (v.qc ? 0.0 : 0.017 * v.bn) +
+  const double hbm = hbm_bytes / 6.6e6 / (0.88 + 0.12 * in_flight);
+  const double l2 = runs * v.cg * v.split * bytes / 15e6;
+  return std::max(std::max(sm, alone), std::max(hbm, l2)) + 0.0079 * v.bn / v.split + (v.qc ? 0.0 : 0.017 * v.bn) +
          (turns - 1.0) * 7.2 * (v.split > 1 ? 1.0 : 0.3) + (v.split > 1 ? 0.18 + 0.039 * v.split + 0.019 * v.bn : 0.0);
 }
 
-GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
+GaPlan ga_choose(const GemmActProblem* ps, int count, bool vec) {
   GaPlan best{false, 16, 1, 1};
   double best_cost = 1e300;
-  const int64_t kb = std::max<int64_t>((K + GA_BK - 1) / GA_BK, 1);
+  int64_t kb = INT32_MAX;
+  for (int i = 0; i < count; ++i) kb = std::min<int64_t>(kb, std::max(1, (ps[i].K + GA_BK - 1) / GA_BK));
   for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
     for (int bn = qc ? 64 : 16; bn <= 256; bn = bn < 64 ? bn + 16 : bn * 2) {
       for (int split = 1; split <= (bn == 256 ? 1 : 8) && split <= kb; split *= 2) {
         const GaPlan v{qc != 0, bn, bn == 256 ? 2 : 1, split};
-        const double c = ga_cost(v, M, N, K);
+        const double c = ga_cost(v, ps, count);
         if (c < best_cost) {
           best_cost = c;
           best = v;
@@ -953,16 +1077,20 @@ GaPlan ga_choose(int64_t M, int64_t N, int64_t K, bool vec) {
 }
 
 template <int BN, int CG, bool QC>
-cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaStream_t stream) {
+cudaError_t ga_launch(const GaMaps& maps, GaArgs& g, int count, cudaStream_t stream) {
   constexpr int YROWS = BN / CG;
-  const int y_bytes = (a.y_mn || BN != 64 ? YROWS : a.bn) * 128;
-  a.stage_bytes = GA_X_BYTES + y_bytes;
-  const int staging = a.stage_out ? GaShape<BN>::EPILOGUE_WARPS * (a.pre ? 8192 : 4096) : 0;
-  int budget = GA_SMEM - staging;
-  if (BN == 64) budget = 108 * 1024 - staging;
-  a.stages = std::min(GA_MAX_STAGES, budget / a.stage_bytes);
-  int smem = a.stages * a.stage_bytes + staging;
-  if (a.split > 1) smem = std::max(smem, BN * 128 * 4);
+  g.stage_bytes = 0;
+  g.out_bytes = 0;
+  for (int i = 0; i < count; ++i) {
+    g.p[i].tx_bytes = GA_X_BYTES + (g.p[i].y_mn || BN != 64 ? YROWS : g.bn) * 128;
+    g.stage_bytes = std::max(g.stage_bytes, g.p[i].tx_bytes);
+    if (g.stage_out) g.out_bytes = std::max(g.out_bytes, g.p[i].pre ? 8192 : 4096);
+  }
+  const int staging = GaShape<BN>::EPILOGUE_WARPS * g.out_bytes;
+  const int budget = (BN == 64 ? GA_SMEM_HALF : GA_SMEM) - staging;
+  g.stages = std::min(GA_MAX_STAGES, budget / g.stage_bytes);
+  int smem = g.stages * g.stage_bytes + staging;
+  if (g.split > 1) smem = std::max(smem, BN * 128 * 4);
   smem += 1024;
   auto kernel = gemm_act_kernel<BN, CG, QC>;
   static std::atomic<bool> configured[PARALIA_MAX_UNITS] = {};
@@ -974,11 +1102,10 @@ cudaError_t ga_launch(const CUtensorMap (&maps)[4], GemmActKernelArgs& a, cudaSt
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  const int group = CG * a.split;
-  int64_t grid = (int64_t)a.tiles * group;
-  if (a.split == 1) grid = std::min<int64_t>(grid, (BN == 64 ? 2 * GA_SMS : GA_SMS) / CG * CG);
-  return launch_dependent(kernel, (int)grid, GaShape<BN>::THREADS, smem, group, stream, maps[0], maps[1], maps[2], maps[3],
-                          a);
+  const int group = CG * g.split;
+  int64_t grid = (int64_t)g.tiles * group;
+  if (g.split == 1) grid = std::min<int64_t>(grid, (BN == 64 ? 2 * GA_SMS : GA_SMS) / CG * CG);
+  return launch_dependent(kernel, (int)grid, GaShape<BN>::THREADS, smem, group, stream, maps, g);
 }
 
 // Whether TMA can read a stored operand of `cols` columns in place.
@@ -993,90 +1120,102 @@ int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int
   return ((rows + 7) / 8 * 8 * cols * 2 + 255) / 256 * 256;
 }
 
-int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStream_t stream) {
-  if (p.M == 0 || p.N == 0) return PARALIA_OK;
-  const bool k_work = p.K > 0;
-  const void* A = p.A;
-  const void* B = p.B;
-  int64_t ldA = p.ldA, ldB = p.ldB;
-  const int64_t a_rows = p.ta ? p.K : p.M, a_cols = p.ta ? p.M : p.K;
-  const int64_t b_rows = p.tb ? p.N : p.K, b_cols = p.tb ? p.K : p.N;
-  if (k_work) {
-    char* s = static_cast<char*>(scratch);
-    AlignCopies c;
-    memset(&c, 0, sizeof(c));
-    int n = 0;
-    auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
-      const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
-      const int64_t ld8 = (rows + 7) / 8 * 8;
-      if (bytes > 0) {
-        c.m[n] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(s), ld, ld8, rows, cols};
-        c.groups[n++] = ld8 / 8 * cols;
-        q = s;
-        ld = ld8;
-        s += bytes;
-      } else if (cols <= 1) {
-        ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
-      }
-    };
-    in_reach(A, ldA, a_rows, a_cols);
-    in_reach(B, ldB, b_rows, b_cols);
-    if (n > 0) {
-      const int64_t blocks = std::min<int64_t>((c.groups[0] + c.groups[1] + 255) / 256, GA_SMS * 16);
-      PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, c));
-    }
-  }
-  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
-  const bool vec = vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) &&
-                   vec16(p.bias, 0);
-  GaPlan v = ga_choose(p.M, p.N, p.K, vec);
+int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream) {
+  GemmActProblem ps[GA_MAX_PROBS];
+  int n = 0;
+  for (int i = 0; i < count; ++i)
+    if (problems[i].M > 0 && problems[i].N > 0) ps[n++] = problems[i];
+  if (n == 0) return PARALIA_OK;
 
-  GemmActKernelArgs a;
-  memset(&a, 0, sizeof(a));
-  a.bias = p.bias; a.C = p.C; a.D = p.D; a.pre = p.pre;
-  a.ldC = p.ldC; a.ldD = p.ldD; a.ldPre = p.ldPre;
-  a.M = p.M; a.N = p.N;
-  a.act = p.act; a.bf16 = p.bf16; a.alpha = p.alpha; a.beta = p.beta;
-  a.vec = vec;
-  a.status = status;
-  a.kblocks = (p.K + GA_BK - 1) / GA_BK;
-  a.split = v.split;
-  a.bn = v.bn;
-  const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
-  const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
-  // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits
-  if (r_tiles * std::max<int64_t>(q_tiles, 16) * 8 > INT32_MAX)
-    return fail(PARALIA_ERR_UNSUPPORTED, "M = %d, N = %d: too many tiles", p.M, p.N);
-  a.tiles = (int32_t)(r_tiles * q_tiles);
-  a.r_tiles = (int32_t)r_tiles;
-  a.q_tiles = (int32_t)q_tiles;
-  // A panel's share of Y is what L2 is to hold on to while X streams past: about 32 MB. At
-  // 8192^3 8 tiles of 256 rows are 850 us, 4 or 16 of them 880; at k = 4096 16 are 850 and 8 865.
-  a.panel = (int32_t)std::min<int64_t>(16, std::max<int64_t>(4, (32 << 20) / ((int64_t)v.bn * std::max(p.K, 1) * 2)));
-  // op(A) is stored with k contiguous if it is a transpose, op(B) if it is not
-  const bool a_k = p.ta != 0, b_k = p.tb == 0;
-  const int yrows = v.bn / v.cg, xrows = 128;
-  CUtensorMap maps[4];   // X, Y, D, pre
-  memset(maps, 0, sizeof(maps));
-  // `inner` x `outer` as stored; `k_major`: inner is k
-  auto operand = [&](CUtensorMap* map, const void* q, int64_t ld, int64_t inner, int64_t outer, bool k_major, int rows,
-                     int32_t* how) -> int {
-    *how = k_major ? GA_K_MAJOR : inner % 64 == 0 && rows >= 64 ? GA_MN_BLOCKS : GA_MN_BOXES;
-    if (!k_work) return PARALIA_OK;
-    if (*how == GA_MN_BLOCKS)
-      return make_tensor_map(map, q, 2, 64, outer, inner / 64, ld * 2, 128, 64, 64, rows / 64);
-    return make_tensor_map(map, q, 2, inner, outer, 1, ld * 2, (uint64_t)ld * outer * 2, 64, k_major ? rows : 64);
+  // operands that TMA cannot address where they are
+  AlignCopies copies;
+  memset(&copies, 0, sizeof(copies));
+  int copied = 0;
+  char* room = static_cast<char*>(scratch);
+  auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
+    const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
+    const int64_t ld8 = (rows + 7) / 8 * 8;
+    if (bytes > 0) {
+      copies.m[copied] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(room), ld, ld8, rows, cols};
+      copies.groups[copied++] = ld8 / 8 * cols;
+      q = room;
+      ld = ld8;
+      room += bytes;
+    } else if (cols <= 1) {
+      ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
+    }
   };
-  PL_TRY(operand(&maps[v.qc ? 1 : 0], A, ldA, a_rows, a_cols, a_k, v.qc ? yrows : xrows, v.qc ? &a.y_mn : &a.x_mn));
-  PL_TRY(operand(&maps[v.qc ? 0 : 1], B, ldB, b_rows, b_cols, b_k, v.qc ? xrows : yrows, v.qc ? &a.x_mn : &a.y_mn));
-  a.stage_out = v.qc && v.split == 1;
-  if (a.stage_out) {
-    PL_TRY(make_tensor_map(&maps[2], p.D, 2, p.M, p.N, 1, p.ldD * 2, (uint64_t)p.ldD * p.N * 2, 64, 32));
-    if (p.pre) PL_TRY(make_tensor_map(&maps[3], p.pre, 2, p.M, p.N, 1, p.ldPre * 2, (uint64_t)p.ldPre * p.N * 2, 64, 32));
+  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
+  bool vec = true;
+  for (int i = 0; i < n; ++i) {
+    GemmActProblem& p = ps[i];
+    vec = vec && vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) && vec16(p.bias, 0);
+    if (p.K == 0) continue;
+    in_reach(p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K);
+    in_reach(p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N);
   }
+  if (copied > 0) {
+    const int64_t blocks = std::min<int64_t>((copies.groups[0] + copies.groups[1] + 255) / 256, GA_SMS * 16);
+    PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, copies));
+  }
+
+  const GaPlan v = ga_choose(ps, n, vec);
+  GaArgs g;
+  GaMaps maps;
+  memset(&g, 0, sizeof(g));
+  memset(&maps, 0, sizeof(maps));
+  g.bn = v.bn;
+  g.split = v.split;
+  g.status = status;
+  g.stage_out = v.qc && v.split == 1;
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i) {
+    const GemmActProblem& p = ps[i];
+    GaProb& a = g.p[i];
+    a.bias = p.bias; a.C = p.C; a.D = p.D; a.pre = p.pre;
+    a.ldC = p.ldC; a.ldD = p.ldD; a.ldPre = p.ldPre;
+    a.M = p.M; a.N = p.N;
+    a.act = p.act; a.bf16 = p.bf16; a.alpha = p.alpha; a.beta = p.beta;
+    a.vec = vec;
+    a.kblocks = (p.K + GA_BK - 1) / GA_BK;
+    a.tile0 = (int32_t)tiles;
+    const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
+    const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
+    // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits
+    if (r_tiles * std::max<int64_t>(q_tiles, 16) * 16 > INT32_MAX)
+      return fail(PARALIA_ERR_UNSUPPORTED, "M = %d, N = %d: too many tiles", p.M, p.N);
+    a.r_tiles = (int32_t)r_tiles;
+    a.q_tiles = (int32_t)q_tiles;
+    tiles += r_tiles * q_tiles;
+    // A panel's share of Y is what L2 is to hold on to while X streams past: about 32 MB. At
+    // 8192^3 8 tiles of 256 rows are 850 us, 4 or 16 of them 880; at k = 4096 16 are 850 and 8 865.
+    a.panel = (int32_t)std::min<int64_t>(16, std::max<int64_t>(4, (32 << 20) / ((int64_t)v.bn * std::max(p.K, 1) * 2)));
+    // op(A) is stored with k contiguous if it is a transpose, op(B) if it is not
+    const bool a_k = p.ta != 0, b_k = p.tb == 0;
+    const int yrows = v.bn / v.cg, xrows = 128;
+    // `inner` x `outer` as stored; `k_major`: inner is k
+    auto operand = [&](CUtensorMap* map, const void* q, int64_t ld, int64_t inner, int64_t outer, bool k_major, int rows,
+                       int32_t* how) -> int {
+      *how = k_major ? GA_K_MAJOR : inner % 64 == 0 && rows >= 64 ? GA_MN_BLOCKS : GA_MN_BOXES;
+      if (p.K == 0) return PARALIA_OK;
+      if (*how == GA_MN_BLOCKS)
+        return make_tensor_map(map, q, 2, 64, outer, inner / 64, ld * 2, 128, 64, 64, rows / 64);
+      return make_tensor_map(map, q, 2, inner, outer, 1, ld * 2, (uint64_t)ld * outer * 2, 64, k_major ? rows : 64);
+    };
+    PL_TRY(operand(v.qc ? &maps.y[i] : &maps.x[i], p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K, a_k,
+                   v.qc ? yrows : xrows, v.qc ? &a.y_mn : &a.x_mn));
+    PL_TRY(operand(v.qc ? &maps.x[i] : &maps.y[i], p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N, b_k,
+                   v.qc ? xrows : yrows, v.qc ? &a.x_mn : &a.y_mn));
+    if (g.stage_out) {
+      PL_TRY(make_tensor_map(&maps.d[i], p.D, 2, p.M, p.N, 1, p.ldD * 2, (uint64_t)p.ldD * p.N * 2, 64, 32));
+      if (p.pre) PL_TRY(make_tensor_map(&maps.pre, p.pre, 2, p.M, p.N, 1, p.ldPre * 2, (uint64_t)p.ldPre * p.N * 2, 64, 32));
+    }
+    if (i == 0) g.tiles0 = (int32_t)tiles;
+  }
+  g.tiles = (int32_t)tiles;
   cudaError_t e = cudaErrorInvalidValue;
 #define GA_CASE(BN, CG, QC) \
-  if ((BN == 64 ? v.bn <= 64 : v.bn == BN) && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, a, stream);
+  if ((BN == 64 ? v.bn <= 64 : v.bn == BN) && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, g, n, stream);
   GA_CASE(64, 1, false)
   GA_CASE(128, 1, false)
   GA_CASE(256, 2, false)
@@ -1088,34 +1227,17 @@ int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStr
   return PARALIA_OK;
 }
 
-int act_grad_chunks(int64_t M, int64_t N) {
-  // a function of the sizes alone, so that the order of the row sums is too: about 1200
-  // blocks, eight for each of 148 SMs, and no run shorter than one column per warp
-  const int64_t row_blocks = (M + AG_ROWS - 1) / AG_ROWS;
-  const int64_t want = row_blocks > 0 ? (1184 + row_blocks - 1) / row_blocks : 1;
-  const int64_t most = std::max<int64_t>(1, (N + AG_WARPS - 1) / AG_WARPS);
-  return (int)std::max<int64_t>(1, std::min(want, most));
-}
-
 cudaError_t launch_act_grad(const ActGradProblem& p, cudaStream_t stream) {
   if (p.M == 0) return cudaSuccess;
-  int chunks = act_grad_chunks(p.M, p.N);
-  const int cols = std::max(1, (p.N + chunks - 1) / chunks);
-  chunks = (p.N + cols - 1) / cols;   // 0 when there are no columns: the sums are 0
-  if (chunks > 0) {
-    const dim3 grid((p.M + AG_ROWS - 1) / AG_ROWS, chunks);
-    const bool vec = vec16(p.dD, p.ldD) && (!p.dZ || vec16(p.dZ, p.ldZ)) &&
-                     (p.act == PARALIA_ACT_NONE || vec16(p.pre, p.ldPre));
-    if (vec) act_grad_kernel<true><<<grid, AG_WARPS * 32, 0, stream>>>(p, cols);
-    else act_grad_kernel<false><<<grid, AG_WARPS * 32, 0, stream>>>(p, cols);
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return e;
-  }
-  if (p.dbias) {
-    act_grad_bias_kernel<<<(p.M + 255) / 256, 256, 0, stream>>>(p, chunks);
-    return cudaGetLastError();
-  }
-  return cudaSuccess;
+  // a function of the sizes alone, so that the order of the row sums is too: as many blocks to a
+  // cluster as there are columns for, eight at most
+  int parts = 1;
+  while (parts < 8 && p.N >= parts * AG_COLS) parts *= 2;
+  const int64_t grid = (p.M + AG_ROWS - 1) / AG_ROWS * (int64_t)parts;
+  const bool vec = vec16(p.dD, p.ldD) && (!p.dZ || vec16(p.dZ, p.ldZ)) &&
+                   (p.act == PARALIA_ACT_NONE || vec16(p.pre, p.ldPre));
+  return launch_dependent(vec ? act_grad_kernel<true> : act_grad_kernel<false>, (int)grid, AG_WARPS * 32, 0, parts, stream,
+                          p, parts);
 }
 
 }  // namespace paralia

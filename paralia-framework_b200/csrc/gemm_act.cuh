@@ -27,25 +27,23 @@ struct GemmActProblem {
 // Bytes of the aligned copy that a stored rows x cols operand needs before TMA can read it; 0 if it
 // is read in place. A multiple of 256.
 int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols);
-// `scratch` (16-byte aligned) holds the copies of A and of B; `status` is the GPU's word for waits
-// that gave up. Returns a PARALIA_* code.
-int launch_gemm_act(const GemmActProblem& p, void* scratch, int* status, cudaStream_t stream);
+// One or two products that do not depend on each other, of the same element type, in one launch; `pre`
+// only with the first. `scratch` (16-byte aligned) holds the copies of operands, at most two in all;
+// `status` is the GPU's word for waits that gave up. Returns a PARALIA_* code.
+int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream);
 
 // dZ <- dD * act'(pre) (dZ may be null; pre is not read for PARALIA_ACT_NONE), and, where
 // dbias is not null, dbias <- row sums of the unrounded product + beta_bias * dbias.
-// `partials` holds act_grad_chunks(M, N) * M floats; it is used when dbias is asked for.
 struct ActGradProblem {
   const void* pre;
   const void* dD;
   void* dZ;
   void* dbias;
-  float* partials;
   int64_t ldPre, ldD, ldZ;
   int32_t M, N;
   int32_t act, bf16;
   float beta_bias;
 };
-int act_grad_chunks(int64_t M, int64_t N);
 cudaError_t launch_act_grad(const ActGradProblem& p, cudaStream_t stream);
 
 }  // namespace paralia

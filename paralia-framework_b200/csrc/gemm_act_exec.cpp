@@ -90,27 +90,24 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   p.ta = is_trans(TransA); p.tb = is_trans(TransB);
   p.act = act; p.bf16 = type == PARALIA_BF16;
   p.alpha = alpha; p.beta = beta;
-  return launch_gemm_act(p, scratch, rt.dev(dev).status_dev, static_cast<cudaStream_t>(stream));
+  return launch_gemm_act(&p, 1, scratch, rt.dev(dev).status_dev, static_cast<cudaStream_t>(stream));
 }
 
 namespace {
 
 // Scratch of the gradient: dZ (M x N, leading dimension a multiple of eight; without an
-// activation the aligned copy of dD where it needs one), then the partial row sums of the bias
-// gradient, then the aligned copies of A and of B where they need one. Only one product runs at
-// a time and each takes one of the two operands, so the copies share their place.
+// activation the aligned copy of dD where it needs one), then the aligned copies of A and of B
+// where they need one.
 struct GradScratch {
-  int64_t ldZ, z_bytes, partial_bytes, copy_bytes, total;
+  int64_t ldZ, z_bytes, total;
 };
 GradScratch grad_scratch(int64_t M, int64_t N, int64_t K, bool ta, bool tb, const void* A, int64_t ldA, const void* B,
                          int64_t ldB) {
   GradScratch g;
   g.ldZ = round_up(std::max<int64_t>(1, M), 8);
   g.z_bytes = round_up(g.ldZ * N * 2, 256);
-  g.partial_bytes = round_up((int64_t)act_grad_chunks(M, N) * M * (int64_t)sizeof(float), 256);
-  g.copy_bytes = std::max(gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K),
-                          gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N));
-  g.total = g.z_bytes + g.partial_bytes + g.copy_bytes;
+  g.total = g.z_bytes + gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K) +
+            gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N);
   return g;
 }
 
@@ -169,23 +166,21 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
     ActGradProblem a;
     memset(&a, 0, sizeof(a));
     a.pre = pre; a.dD = dD; a.dZ = need_z ? base : nullptr; a.dbias = want_bias ? dbias : nullptr;
-    a.partials = reinterpret_cast<float*>(base + g.z_bytes);
     a.ldPre = ldPre; a.ldD = lddD; a.ldZ = g.ldZ;
     a.M = (int32_t)M; a.N = (int32_t)N; a.act = act; a.bf16 = bf16; a.beta_bias = betaBias;
     PL_CUDA(launch_act_grad(a, s));
   }
   const void* dZ = need_z ? base : dD;
   const int64_t ldZ = need_z ? g.ldZ : lddD;
-  void* copies = base + g.z_bytes + g.partial_bytes;
+  void* copies = base + g.z_bytes;
   int* status = rt.dev(dev).status_dev;
 
-  GemmActProblem p;
-  memset(&p, 0, sizeof(p));
-  p.act = PARALIA_ACT_NONE;
-  p.bf16 = bf16;
-  p.alpha = alpha;
+  GemmActProblem ps[2];
+  memset(ps, 0, sizeof(ps));
+  int count = 0;
   if (want_b) {
     // d op(B) = alpha op(A)^T dZ, stored as B is
+    GemmActProblem& p = ps[count++];
     p.D = dB; p.ldD = lddB; p.C = betaB != 0.0f ? dB : nullptr; p.ldC = lddB; p.beta = betaB;
     p.K = alpha != 0.0f ? (int32_t)M : 0;
     if (!tb) {
@@ -195,10 +190,10 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
       p.A = dZ; p.ldA = ldZ; p.ta = 1; p.B = A; p.ldB = ldA; p.tb = ta;
       p.M = (int32_t)N; p.N = (int32_t)K;
     }
-    PL_TRY(launch_gemm_act(p, copies, status, s));
   }
   if (want_a) {
     // d op(A) = alpha dZ op(B)^T, stored as A is
+    GemmActProblem& p = ps[count++];
     p.D = dA; p.ldD = lddA; p.C = betaA != 0.0f ? dA : nullptr; p.ldC = lddA; p.beta = betaA;
     p.K = alpha != 0.0f ? (int32_t)N : 0;
     if (!ta) {
@@ -208,9 +203,13 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
       p.A = B; p.ldA = ldB; p.ta = tb; p.B = dZ; p.ldB = ldZ; p.tb = 1;
       p.M = (int32_t)K; p.N = (int32_t)M;
     }
-    PL_TRY(launch_gemm_act(p, copies, status, s));
   }
-  return PARALIA_OK;
+  for (int i = 0; i < count; ++i) {
+    ps[i].act = PARALIA_ACT_NONE;
+    ps[i].bf16 = bf16;
+    ps[i].alpha = alpha;
+  }
+  return launch_gemm_act(ps, count, copies, status, s);
 }
 
 }  // namespace paralia
