@@ -512,7 +512,8 @@ __device__ __forceinline__ GaTile ga_tile(const GaProb& a, int tile) {
   return t;
 }
 
-template <int BN, int CG, bool QC>
+// TWO: the launch has two products. With one its description is read from constant addresses.
+template <int BN, int CG, bool QC, bool TWO>
 __global__ void __launch_bounds__(GaShape<BN>::THREADS, BN == 64 ? 2 : 1)
 gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaArgs g) {
   extern __shared__ unsigned char smem_raw[];
@@ -585,7 +586,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
     uint32_t phase = 0;              // parity of the ring's round
     bool ok = true;
     for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step) {
-      const int which = tile >= g.tiles0 ? 1 : 0;
+      const int which = TWO && tile >= g.tiles0 ? 1 : 0;
       const GaProb& a = g.p[which];
       const CUtensorMap *map_x = &maps.x[which], *map_y = &maps.y[which];
       const int kb0 = k_begin(a), kb1 = k_end(a);
@@ -654,7 +655,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
           ok = false;
           break;
         }
-        const GaProb& a = g.p[tile >= g.tiles0 ? 1 : 0];
+        const GaProb& a = g.p[TWO && tile >= g.tiles0 ? 1 : 0];
         const int kb0 = k_begin(a), kb1 = k_end(a);
         const uint32_t fmt = a.bf16 ? 1u : 0u;
         const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (a.x_mn ? 1u << 15 : 0u) | (a.y_mn ? 1u << 16 : 0u) |
@@ -692,7 +693,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
     bool ok = true;
     for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step, ++local) {
       const int buf = local & 1;
-      const int which = tile >= g.tiles0 ? 1 : 0;
+      const int which = TWO && tile >= g.tiles0 ? 1 : 0;
       const GaProb& a = g.p[which];
       const GaTile t = ga_tile(a, tile);
       {
@@ -756,7 +757,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
       // A warp sums one column of this CTA's share at a time, a lane four rows of it: 512 contiguous
       // bytes from each CTA. The sums replace this CTA's own share, which nobody else reads.
       const int cols = bn / split;                    // columns of this CTA
-      const GaProb& a = g.p[first_tile >= g.tiles0 ? 1 : 0];
+      const GaProb& a = g.p[TWO && first_tile >= g.tiles0 ? 1 : 0];
       const GaTile t = ga_tile(a, first_tile);
       float* own = reinterpret_cast<float*>(smem) + (int)rank * cols * 128;
       // columns that exist (QC: all, the others are cut off later)
@@ -1062,7 +1063,7 @@ GaPlan ga_choose(const GemmActProblem* ps, int count, bool vec) {
   return best;
 }
 
-template <int BN, int CG, bool QC>
+template <int BN, int CG, bool QC, bool TWO>
 cudaError_t ga_launch(const GaMaps& maps, GaArgs& g, int count, cudaStream_t stream) {
   constexpr int YROWS = BN / CG;
   g.stage_bytes = 0;
@@ -1078,7 +1079,7 @@ cudaError_t ga_launch(const GaMaps& maps, GaArgs& g, int count, cudaStream_t str
   int smem = g.stages * g.stage_bytes + staging;
   if (g.split > 1) smem = std::max(smem, BN * 128 * 4);
   smem += 1024;
-  auto kernel = gemm_act_kernel<BN, CG, QC>;
+  auto kernel = gemm_act_kernel<BN, CG, QC, TWO>;
   static std::atomic<bool> configured[PARALIA_MAX_UNITS] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1201,7 +1202,8 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
   g.tiles = (int32_t)tiles;
   cudaError_t e = cudaErrorInvalidValue;
 #define GA_CASE(BN, CG, QC) \
-  if ((BN == 64 ? v.bn <= 64 : v.bn == BN) && v.cg == CG && v.qc == QC) e = ga_launch<BN, CG, QC>(maps, g, n, stream);
+  if ((BN == 64 ? v.bn <= 64 : v.bn == BN) && v.cg == CG && v.qc == QC)                                     \
+    e = n == 2 ? ga_launch<BN, CG, QC, true>(maps, g, n, stream) : ga_launch<BN, CG, QC, false>(maps, g, n, stream);
   GA_CASE(64, 1, false)
   GA_CASE(128, 1, false)
   GA_CASE(256, 2, false)
