@@ -235,15 +235,19 @@ def _ptr(x) -> int:
         return 0
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return int(x.data_ptr())
+    data_ptr = getattr(x, "data_ptr", None)
+    if data_ptr is not None:
+        return int(data_ptr())
     if hasattr(x, "ctypes"):
         return int(x.ctypes.data)
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+_FLAGS = {ch: ch.encode() for ch in "NTCntc"}
+
+
 def _c(ch: str) -> bytes:
-    return ch.encode()[:1]
+    return _FLAGS.get(ch) or ch.encode()[:1]
 
 
 def make_ctl(T: int = 0, units=None, cache_limit: int = 0, exec_streams: int = 0,

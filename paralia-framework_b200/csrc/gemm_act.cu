@@ -382,7 +382,8 @@ __device__ __forceinline__ void ga_staged_tile(const GaProb& a, const CUtensorMa
                                                int r_first, int cols, int lane) {
   const uint32_t row = out + lane * 128;
   const int64_t n = min((int64_t)r_first + lane, (int64_t)a.N - 1);   // a column that exists; its copy is cut off
-  const int last = min(cols, ((a.M - q + 63) / 64) * 64);              // 64 rows of which none exists are left out
+  const int left = a.M - q;
+  const int last = left >= cols ? cols : (left + 63) / 64 * 64;        // 64 rows of which none exists are left out
   if (last <= 0) return;
   uint32_t v[16];
   uint4 c0 = ga_load_c8(a, q, n), c1 = ga_load_c8(a, (int64_t)q + 8, n);
@@ -512,6 +513,13 @@ __device__ __forceinline__ GaTile ga_tile(const GaProb& a, int tile) {
   return t;
 }
 
+// The tile of place `place` in the round that starts at tile `base`. The last, incomplete round is dealt
+// out from the other end: of two products the one with more k comes first, so that the places at
+// the end have had less to do.
+__device__ __forceinline__ int ga_number(int base, int place, int step, int tiles) {
+  return base + (base + step > tiles ? step - 1 - place : place);
+}
+
 // TWO: the launch has two products. With one its description is read from constant addresses.
 template <int BN, int CG, bool QC, bool TWO>
 __global__ void __launch_bounds__(GaShape<BN>::THREADS, BN == 64 ? 2 : 1)
@@ -530,7 +538,8 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
   const uint32_t rank = (CG == 2 || g.split > 1) ? cluster_rank() : 0;
   const int split = CG == 1 ? g.split : 1;
   const int group = CG * split;                        // CTAs that share a tile
-  const int first_tile = blockIdx.x / group, tile_step = gridDim.x / group;
+  const int place = blockIdx.x / group, tile_step = gridDim.x / group;
+  const int first_tile = ga_number(0, place, tile_step, g.tiles);
   // this CTA's run of a product's k blocks
   auto k_begin = [&](const GaProb& a) { return split > 1 ? (int)((int64_t)a.kblocks * rank / split) : 0; };
   auto k_end = [&](const GaProb& a) { return split > 1 ? (int)((int64_t)a.kblocks * (rank + 1) / split) : a.kblocks; };
@@ -585,7 +594,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
     int s = 0, filled = 0;           // stage, and how many stages have been filled at all (capped)
     uint32_t phase = 0;              // parity of the ring's round
     bool ok = true;
-    for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step) {
+    for (int base = 0, tile; ok && (tile = ga_number(base, place, tile_step, g.tiles)) < g.tiles; base += tile_step) {
       const int which = TWO && tile >= g.tiles0 ? 1 : 0;
       const GaProb& a = g.p[which];
       const CUtensorMap *map_x = &maps.x[which], *map_y = &maps.y[which];
@@ -648,7 +657,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
       uint32_t phase = 0;
       int local = 0;
       bool ok = true;
-      for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step, ++local) {
+      for (int base = 0, tile; ok && (tile = ga_number(base, place, tile_step, g.tiles)) < g.tiles; base += tile_step, ++local) {
         const int buf = local & 1;
         if (local >= 2 && !warp_wait(&ctl->acc_empty[buf], (uint32_t)(((local >> 1) - 1) & 1), abort_flag)) {
           if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_TMEM_WAIT_TIMEOUT); }
@@ -691,7 +700,7 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
     const int part_cols = bn / (EW / 4);
     int local = 0;
     bool ok = true;
-    for (int tile = first_tile; tile < g.tiles && ok; tile += tile_step, ++local) {
+    for (int base = 0, tile; ok && (tile = ga_number(base, place, tile_step, g.tiles)) < g.tiles; base += tile_step, ++local) {
       const int buf = local & 1;
       const int which = TWO && tile >= g.tiles0 ? 1 : 0;
       const GaProb& a = g.p[which];
@@ -994,6 +1003,8 @@ cudaError_t launch_dependent(void (*kernel)(P...), int grid, int threads, int sm
   return cudaLaunchKernelEx(&cfg, kernel, std::forward<Q>(args)...);
 }
 
+inline int64_t ga_kblocks(int64_t k) { return (k + GA_BK - 1) / GA_BK; }
+
 // One way to run a product: orientation, tile, split of k.
 struct GaPlan {
   bool qc;
@@ -1001,6 +1012,8 @@ struct GaPlan {
 };
 
 constexpr int GA_SMS = 148;
+
+std::atomic<unsigned> ga_generation{1};
 
 int64_t ga_tiles(const GaPlan& v, int64_t M, int64_t N) {
   const int64_t R = v.qc ? N : M, Q = v.qc ? M : N;
@@ -1016,7 +1029,7 @@ double ga_cost(const GaPlan& v, const GemmActProblem* ps, int count) {
   double hbm_bytes = 0.0, runs = 0.0;
   for (int i = 0; i < count; ++i) {
     const int64_t t = ga_tiles(v, ps[i].M, ps[i].N);
-    const int64_t r = ((ps[i].K + GA_BK - 1) / GA_BK + v.split - 1) / v.split;   // k blocks of a CTA
+    const int64_t r = (ga_kblocks(ps[i].K) + v.split - 1) / v.split;   // k blocks of a CTA
     tiles += t;
     runs += (double)t * r;
     run = std::max(run, r);
@@ -1047,7 +1060,7 @@ GaPlan ga_choose(const GemmActProblem* ps, int count, bool vec) {
   GaPlan best{false, 16, 1, 1};
   double best_cost = 1e300;
   int64_t kb = INT32_MAX;
-  for (int i = 0; i < count; ++i) kb = std::min<int64_t>(kb, std::max(1, (ps[i].K + GA_BK - 1) / GA_BK));
+  for (int i = 0; i < count; ++i) kb = std::min(kb, std::max<int64_t>(1, ga_kblocks(ps[i].K)));
   for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
     for (int bn = qc ? 64 : 16; bn <= 256; bn = bn < 64 ? bn + 16 : bn * 2) {
       for (int split = 1; split <= (bn == 256 ? 1 : 8) && split <= kb; split *= 2) {
@@ -1080,14 +1093,16 @@ cudaError_t ga_launch(const GaMaps& maps, GaArgs& g, int count, cudaStream_t str
   if (g.split > 1) smem = std::max(smem, BN * 128 * 4);
   smem += 1024;
   auto kernel = gemm_act_kernel<BN, CG, QC, TWO>;
-  static std::atomic<bool> configured[PARALIA_MAX_UNITS] = {};
+  // once per GPU, and again after the library has been shut down
+  static std::atomic<unsigned> configured[PARALIA_MAX_UNITS] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (!configured[dev]) {
+  const unsigned now = ga_generation;
+  if (configured[dev] != now) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, GA_SMEM + 1024);
     if (e != cudaSuccess) return e;
-    configured[dev] = true;
+    configured[dev] = now;
   }
   const int group = CG * g.split;
   int64_t grid = (int64_t)g.tiles * group;
@@ -1102,6 +1117,8 @@ bool ga_in_place(const void* p, int64_t ld, int64_t cols) {
 
 }  // namespace
 
+void gemm_act_forget_configuration() { ++ga_generation; }
+
 int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || ga_in_place(p, ld, cols)) return 0;
   return ((rows + 7) / 8 * 8 * cols * 2 + 255) / 256 * 256;
@@ -1113,6 +1130,7 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
   for (int i = 0; i < count; ++i)
     if (problems[i].M > 0 && problems[i].N > 0) ps[n++] = problems[i];
   if (n == 0) return PARALIA_OK;
+  if (n == 2 && ps[1].K > ps[0].K && !ps[0].pre) std::swap(ps[0], ps[1]);
 
   // operands that TMA cannot address where they are
   AlignCopies copies;
@@ -1164,12 +1182,12 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
     a.M = p.M; a.N = p.N;
     a.act = p.act; a.bf16 = p.bf16; a.alpha = p.alpha; a.beta = p.beta;
     a.vec = vec;
-    a.kblocks = (p.K + GA_BK - 1) / GA_BK;
+    a.kblocks = (int32_t)ga_kblocks(p.K);
     a.tile0 = (int32_t)tiles;
     const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
     const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
-    // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits
-    if (r_tiles * std::max<int64_t>(q_tiles, 16) * 16 > INT32_MAX)
+    // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits; clusters have up to 8 CTAs
+    if (r_tiles * std::max<int64_t>(q_tiles, 16) > INT32_MAX / 16 || tiles + r_tiles * q_tiles > INT32_MAX / 16)
       return fail(PARALIA_ERR_UNSUPPORTED, "M = %d, N = %d: too many tiles", p.M, p.N);
     a.r_tiles = (int32_t)r_tiles;
     a.q_tiles = (int32_t)q_tiles;
@@ -1194,8 +1212,10 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
     PL_TRY(operand(v.qc ? &maps.x[i] : &maps.y[i], p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N, b_k,
                    v.qc ? xrows : yrows, v.qc ? &a.x_mn : &a.y_mn));
     if (g.stage_out) {
-      PL_TRY(make_tensor_map(&maps.d[i], p.D, 2, p.M, p.N, 1, p.ldD * 2, (uint64_t)p.ldD * p.N * 2, 64, 32));
-      if (p.pre) PL_TRY(make_tensor_map(&maps.pre, p.pre, 2, p.M, p.N, 1, p.ldPre * 2, (uint64_t)p.ldPre * p.N * 2, 64, 32));
+      // (the leading dimension of a single column has no meaning and any value)
+      const int64_t ld1 = ((int64_t)p.M + 7) / 8 * 8, ldD = p.N > 1 ? p.ldD : ld1, ldPre = p.N > 1 ? p.ldPre : ld1;
+      PL_TRY(make_tensor_map(&maps.d[i], p.D, 2, p.M, p.N, 1, ldD * 2, (uint64_t)ldD * p.N * 2, 64, 32));
+      if (p.pre) PL_TRY(make_tensor_map(&maps.pre, p.pre, 2, p.M, p.N, 1, ldPre * 2, (uint64_t)ldPre * p.N * 2, 64, 32));
     }
     if (i == 0) g.tiles0 = (int32_t)tiles;
   }

@@ -32,6 +32,9 @@ int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int
 // `status` is the GPU's word for waits that gave up. Returns a PARALIA_* code.
 int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream);
 
+// Makes every GPU's kernels be configured anew at their next launch (library shutdown).
+void gemm_act_forget_configuration();
+
 // dZ <- dD * act'(pre) (dZ may be null; pre is not read for PARALIA_ACT_NONE), and, where
 // dbias is not null, dbias <- row sums of the unrounded product + beta_bias * dbias.
 struct ActGradProblem {

@@ -12,6 +12,7 @@
 
 #include "autotune.hpp"
 #include "dgemm_tile.cuh"
+#include "gemm_act.cuh"
 #include "level1.cuh"
 #include "sgemm_tile.cuh"
 
@@ -382,6 +383,7 @@ int Runtime::finalize() {
     }
   }
   ddot_noalloc_forget_addresses();
+  gemm_act_forget_configuration();
   devs_.clear();
   ndev_ = 0;
   inited_ = false;

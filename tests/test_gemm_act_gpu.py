@@ -364,3 +364,44 @@ def test_grad_against_differences(pl, act):
         t = float(t[i] if t.dim() == 1 else t[i, j])
         # the differences' own error: h^2/6 times a third derivative (below 3 in sum here) and rounding
         assert abs(float(out[key].t[i, j]) - diff) <= t + h * h * 16 + 1e-9, (key, i, j)
+
+
+def test_offsets_beyond_32_bits(pl):
+    # D has 4.6e9 entries; the last columns, rows and a few in between are looked at
+    import torch
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    M, N, K = 65544, 70001, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    A = torch.randint(-2, 3, (M, K), generator=g, device="cuda").to(torch.bfloat16)     # K x M, transposed
+    B = torch.randint(-2, 3, (N, K), generator=g, device="cuda").to(torch.bfloat16)     # K x N
+    D = torch.full((N, M), float("nan"), dtype=torch.bfloat16, device="cuda")
+    pl.tile_gemm_act(0, pl.BF16, "T", "N", M, N, K, 1.0, A, K, B, K, 0.0, None, M, D, M)
+    torch.cuda.synchronize()
+    pl.tile_status(0)
+    cols = torch.tensor([0, 1, 255, 256, 32767, 32768, 40000, 65535, 65536, N - 2, N - 1], device="cuda")
+    want = (B[cols].float() @ A.float().T).to(torch.bfloat16)
+    assert torch.equal(D[cols], want)
+    assert bool(torch.isfinite(D[:, M - 1].float()).all()) and bool(torch.isfinite(D[:, 0].float()).all())
+    rows = torch.tensor([0, 127, 128, 30001, M - 1], device="cuda")
+    assert torch.equal(D[:, rows], (B.float() @ A[rows].float().T).to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("N", [1, 40])
+def test_leading_dimensions_of_single_columns(pl, N):
+    # a single column may have any leading dimension, a wide gap between columns is jumped over
+    import torch
+    d = _defs()
+    M, K = 264, 72
+    g = torch.Generator(device="cuda").manual_seed(8)
+    ld = 1 << 40 if N == 1 else 100_000
+    A = torch.randint(-2, 3, (M, K), generator=g, device="cuda").to(torch.bfloat16)
+    B = torch.randint(-2, 3, (N, K), generator=g, device="cuda").to(torch.bfloat16)
+    D = torch.zeros((N - 1) * (ld if N > 1 else 0) + M, dtype=torch.bfloat16, device="cuda")
+    P = torch.zeros_like(D)
+    pl.tile_gemm_act(0, pl.BF16, "T", "N", M, N, K, 1.0, A, K, B, ld if N == 1 else K, 0.0, None, ld, D, ld, pre=P, ldPre=ld)
+    torch.cuda.synchronize()
+    want = (B.float() @ A.float().T).to(torch.bfloat16)
+    for buf in (D, P):
+        got = buf[:M].reshape(1, M) if N == 1 else torch.as_strided(buf, (N, M), (ld, 1))
+        assert torch.equal(got, want)
