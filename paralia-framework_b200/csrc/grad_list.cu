@@ -5,8 +5,8 @@
 // the scaling. The list travels in the kernel's parameters (no copy, nothing kept between
 // calls, capturable). It is cut into units of 2048 elements and block b of G takes the b-th of G
 // equal runs of units, so what a block has of one tensor is one contiguous span (chunks dealt out
-// in turn, with a search for the tensor of each, read 2 GB of BF16 in 365 us). The order of every
-// sum is a function of the list alone.
+// in turn, with a search for the tensor of each, read 2 GB of BF16 in 365 us; this takes 302, 6.6
+// TB/s). The order of every sum is a function of the list alone.
 //
 // Squares: of FP32 elements they are summed in FP64 throughout (a conversion and an FMA an
 // element, which the FP64 pipe keeps up with at HBM speed). Of 16-bit elements the eight of
