@@ -474,6 +474,18 @@ __device__ __forceinline__ void ga_direct_tile(const GaProb& a, uint32_t taddr, 
       cx[j] = c[j];
     }
     if (at + 16 < last) fetch(at + 16);
+    if (!a.C && !a.pre && at + 16 <= last) {
+      // the common case without a question for every element
+      uint16_t o[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) store16(&o[j], 0, act_value<ACT>(z[j]), bf);
+      if (in) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) dp[j * a.ldD] = o[j];
+      }
+      dp += 16 * a.ldD;
+      continue;
+    }
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
       float d = act_value<ACT>(z[j]);
