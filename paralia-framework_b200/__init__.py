@@ -243,6 +243,15 @@ def _ptr(x) -> int:
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
+def _dev_ptr(x) -> int:
+    """Address of an operand of the mixed-precision routines, which take GPU memory only."""
+    if x is None or isinstance(x, int):
+        return x or 0
+    if not getattr(x, "is_cuda", False):
+        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
+    return x.data_ptr()
+
+
 _FLAGS = {ch: ch.encode() for ch in "NTCntc"}
 
 
@@ -441,8 +450,8 @@ def tile_ddot_noalloc(dev, N, x, incx, y, incy, result_dev, stream: int = 0) -> 
 
 
 def tile_gemm_act_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB) -> int:
-    return int(lib().PARALiA_tile_gemm_act_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _ptr(A), ldA,
-                                                         _ptr(B), ldB))
+    return int(lib().PARALiA_tile_gemm_act_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _dev_ptr(A), ldA,
+                                                         _dev_ptr(B), ldB))
 
 
 def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, beta, Cm, ldC, D, ldD,
@@ -450,14 +459,14 @@ def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, bet
                   scratch_bytes: int = 0, stream: int = 0) -> None:
     """``Z = alpha*op(A)*op(B) + bias``, ``pre <- Z``, ``D <- act(Z) + beta*Cm``, FP16 or BF16 (``type``),
     column-major, on the caller's stream. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _ptr(A), ldA,
-                                       _ptr(B), ldB, _ptr(bias), act, beta, _ptr(Cm), ldC, _ptr(D), ldD,
-                                       _ptr(pre), ldPre, _ptr(scratch), scratch_bytes))
+    _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A), ldA,
+                                       _dev_ptr(B), ldB, _dev_ptr(bias), act, beta, _dev_ptr(Cm), ldC, _dev_ptr(D), ldD,
+                                       _dev_ptr(pre), ldPre, _dev_ptr(scratch), scratch_bytes))
 
 
 def tile_gemm_act_grad_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB, act) -> int:
-    return int(lib().PARALiA_tile_gemm_act_grad_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _ptr(A), ldA,
-                                                              _ptr(B), ldB, act))
+    return int(lib().PARALiA_tile_gemm_act_grad_scratch_bytes(type, _c(TransA), _c(TransB), M, N, K, _dev_ptr(A), ldA,
+                                                              _dev_ptr(B), ldB, act))
 
 
 def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, act, pre, ldPre, dD, lddD,
@@ -466,10 +475,10 @@ def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB
                        stream: int = 0) -> None:
     """Gradient of ``tile_gemm_act``: ``dA``, ``dB`` and ``dbias`` (each may be None) from the gradient ``dD``
     of its result and the pre-activation ``pre`` it kept. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _ptr(A),
-                                            ldA, _ptr(B), ldB, act, _ptr(pre), ldPre, _ptr(dD), lddD, betaA,
-                                            _ptr(dA), lddA, betaB, _ptr(dB), lddB, betaBias, _ptr(dbias),
-                                            _ptr(scratch), scratch_bytes))
+    _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A),
+                                            ldA, _dev_ptr(B), ldB, act, _dev_ptr(pre), ldPre, _dev_ptr(dD), lddD, betaA,
+                                            _dev_ptr(dA), lddA, betaB, _dev_ptr(dB), lddB, betaBias, _dev_ptr(dbias),
+                                            _dev_ptr(scratch), scratch_bytes))
 
 
 _TYPE_OF = {"float32": F32, "float16": F16, "bfloat16": BF16}
@@ -516,22 +525,22 @@ def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
 def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of a list of tensors: ``norm`` (float32) and ``sumsq`` (float64, its square) are device
     scalars, either may be None. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _ptr(scratch),
-                                        _ptr(sumsq), _ptr(norm)))
+    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _dev_ptr(scratch),
+                                        _dev_ptr(sumsq), _dev_ptr(norm)))
 
 
 def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of the list, then every tensor times ``max_norm / norm`` where that is below 1, in place or
     to the list's ``out``. No counterpart in the reference."""
     _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                        grads.out_type, max_norm, _ptr(scratch), _ptr(sumsq), _ptr(norm)))
+                                        grads.out_type, max_norm, _dev_ptr(scratch), _dev_ptr(sumsq), _dev_ptr(norm)))
 
 
 def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:
     """The scaling half of ``tile_grad_clip`` from a squared norm in device memory (the sum over several
     GPUs' lists). No counterpart in the reference."""
     _check(lib().PARALiA_tile_grad_scale(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                         grads.out_type, _ptr(sumsq), max_norm, _ptr(norm)))
+                                         grads.out_type, _dev_ptr(sumsq), max_norm, _dev_ptr(norm)))
 
 
 def malloc(nbytes: int, loc: int) -> int:

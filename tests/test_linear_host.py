@@ -137,6 +137,17 @@ def test_tensor_list_checks(pl):
     assert list(x.n) == [3, 0] and list(x.type) == [pl.BF16, pl.F16] and x.g_out is None
 
 
+def test_host_memory_is_refused(pl):
+    import numpy as np
+    import torch
+    for x in (torch.zeros(1024, dtype=torch.bfloat16), np.zeros(1024, dtype=np.float16)):
+        _refused(pl, _call, A=x)
+        _refused(pl, _call, D=x)
+        _refused(pl, _grad, dbias=x)
+        with pytest.raises(pl.ParaliaError):
+            pl.tile_grad_norm(0, pl.TensorList([]), x, norm=D)
+
+
 def test_scratch_sizes(pl):
     lst = pl.TensorList([])
     assert pl.tile_grad_norm_scratch_bytes(lst) >= 8
