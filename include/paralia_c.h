@@ -306,8 +306,9 @@ int PARALiA_tile_ddot_noalloc(int dev, void* stream, int64_t N,
  * pointers are device pointers of that GPU, PARALiA_tile_status reports a wait that gave up.
  * They allocate nothing; what scratch they need the caller brings. Two calls that may overlap on
  * the GPU (two streams, two captured graphs) need scratch of their own each. All of them can be
- * captured into a graph, after a first call of any tile routine on that GPU has set it up. They
- * have no counterpart in the reference, whose operations are FP64 and FP32 BLAS. */
+ * captured into a graph once a call has set the GPU up (any routine that computes on it; the first
+ * call inside a capture is refused with PARALIA_ERR_UNSUPPORTED). They have no counterpart in the
+ * reference, whose operations are FP64 and FP32 BLAS. */
 #define PARALIA_F32  0
 #define PARALIA_F16  1
 #define PARALIA_BF16 2

@@ -80,8 +80,7 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
-  PL_TRY(rt.ensure_device(dev));
-  PL_CUDA(cudaSetDevice(dev));
+  PL_TRY(rt.enter_tile_call(dev, static_cast<cudaStream_t>(stream)));
   GemmActProblem p;
   memset(&p, 0, sizeof(p));
   p.A = A; p.B = B; p.bias = bias; p.C = beta != 0.0f ? C : nullptr; p.D = D; p.pre = pre;
@@ -152,8 +151,7 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
-  PL_TRY(rt.ensure_device(dev));
-  PL_CUDA(cudaSetDevice(dev));
+  PL_TRY(rt.enter_tile_call(dev, static_cast<cudaStream_t>(stream)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = type == PARALIA_BF16;
 

@@ -92,11 +92,10 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
   return PARALIA_OK;
 }
 
-int enter(int dev) {
+int enter(int dev, void* stream) {
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
-  PL_TRY(rt.ensure_device(dev));
-  PL_CUDA(cudaSetDevice(dev));
+  PL_TRY(rt.enter_tile_call(dev, static_cast<cudaStream_t>(stream)));
   return PARALIA_OK;
 }
 
@@ -125,7 +124,7 @@ int exec_tile_grad_norm(int dev, void* stream, int count, const void* const* g, 
   PL_TRY(check_scratch(scratch));
   if (!sumsq && !norm) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq and norm");
   DeviceGuard guard;
-  PL_TRY(enter(dev));
+  PL_TRY(enter(dev, stream));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int used = 0;
   PL_CUDA(launch_grad_sumsq(l, static_cast<double*>(scratch), &used, s));
@@ -142,7 +141,7 @@ int exec_tile_grad_clip(int dev, void* stream, int count, const void* const* g, 
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   PL_TRY(check_scratch(scratch));
   DeviceGuard guard;
-  PL_TRY(enter(dev));
+  PL_TRY(enter(dev, stream));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int used = 0;
   PL_CUDA(launch_grad_sumsq(l, static_cast<double*>(scratch), &used, s));
@@ -159,7 +158,7 @@ int exec_tile_grad_scale(int dev, void* stream, int count, const void* const* g,
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   if (!sumsq) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq");
   DeviceGuard guard;
-  PL_TRY(enter(dev));
+  PL_TRY(enter(dev, stream));
   // one partial sum is only read
   PL_CUDA(launch_grad_scale(l, const_cast<double*>(sumsq), 1, max_norm, nullptr, norm, static_cast<cudaStream_t>(stream)));
   return PARALIA_OK;

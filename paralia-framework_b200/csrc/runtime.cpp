@@ -248,6 +248,25 @@ int Runtime::ensure_device(int d) {
   return PARALIA_OK;
 }
 
+int Runtime::enter_tile_call(int d, cudaStream_t stream) {
+  if (d < 0 || d >= ndev_) return fail(PARALIA_ERR_INVALID_ARG, "GPU id %d out of range", d);
+  bool ready;
+  {
+    std::lock_guard<std::mutex> lk(device_mutex_);
+    ready = devs_[d].ready;
+  }
+  PL_CUDA(cudaSetDevice(d));
+  if (ready) return PARALIA_OK;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing(stream, &capture);
+  if (e != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return fail(PARALIA_ERR_UNSUPPORTED, "GPU %d has not been used yet and a stream is being captured: make a first "
+                "call before the capture", d);
+  }
+  return ensure_device(d);
+}
+
 int Runtime::ensure_slab(int d, size_t bytes, double* alloc_ms) {
   DeviceCtx& c = devs_[d];
   if (c.slab_bytes >= bytes) return PARALIA_OK;

@@ -85,6 +85,9 @@ class Runtime {
   bool peer_ok(int a, int b) const { return a == b || peer_[a][b]; }
   // Make sure streams/status words of GPU d exist.
   int ensure_device(int d);
+  // The same for a call on the caller's stream, which is then the current device's. Setting a GPU up
+  // allocates, which a stream being captured does not allow: refused there, and the capture stays whole.
+  int enter_tile_call(int d, cudaStream_t stream);
   // Grow (never shrink) the slab of GPU d to at least `bytes`.
   int ensure_slab(int d, size_t bytes, double* alloc_ms);
   int free_slab(int d);

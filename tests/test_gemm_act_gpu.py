@@ -171,7 +171,7 @@ def test_streams_graphs_and_repeats(pl):
     """Two captured graphs with scratch of their own, replayed on their streams after new inputs."""
     import torch
     d = _defs()
-    pl.tile_status(0)
+    pl.fill_f32(torch.zeros(1, device="cuda"), 1, 0, 0, 0)      # sets the GPU up
     cases = []
     for i, (M, N, K, off) in enumerate(((300, 257, 190, 0), (1000, 3, 515, 1))):
         g = torch.Generator(device="cuda").manual_seed(i)

@@ -101,7 +101,7 @@ def test_training_step(pl, dtype, shape):
 def test_captured_step_follows_new_inputs(pl):
     import torch
     import linear_defs as d
-    pl.tile_status(0)
+    pl.fill_f32(torch.zeros(1, device="cuda"), 1, 0, 0, 0)      # sets the GPU up
     st = torch.cuda.Stream()
     b = Block(pl, d, 130, 200, 515, "bf16", stream=st.cuda_stream)
     graph = torch.cuda.CUDAGraph()
@@ -175,7 +175,6 @@ def test_calls_from_two_threads(pl):
     """Two host threads, a stream and scratch each, at the same time: the bits of one after the other."""
     import torch
     import linear_defs as d
-    pl.tile_status(0)
     streams = [torch.cuda.Stream() for _ in range(2)]
     blocks = [Block(pl, d, 200 + 37 * i, 264, 520, "bf16", seed=i, stream=streams[i].cuda_stream) for i in range(2)]
     torch.cuda.synchronize()
@@ -227,3 +226,75 @@ def test_norm_over_two_lists_then_scale(pl):
         for t, o in zip(l, b):
             v = o.double() * (2.5 / want)
             assert bool(((t.double() - v).abs() <= (2.0 ** -8 + 2.0 ** -20) * v.abs()).all())
+
+
+FRESH = r"""
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+import __graft_entry__ as e
+pl = e.load_package()
+pl.lib()
+
+def ops(stream, M):
+    N, K = 260, 203
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    A, B, D, P = torch.randn(M, K, **bf), torch.randn(N, K, **bf), torch.zeros(N, M, **bf), torch.zeros(N, M, **bf)
+    dA, dB, db = torch.zeros_like(A), torch.zeros_like(B), torch.zeros(M, **bf)
+    n = max(pl.tile_gemm_act_scratch_bytes(pl.BF16, "T", "N", M, N, K, A, K, B, K),
+            pl.tile_gemm_act_grad_scratch_bytes(pl.BF16, "T", "N", M, N, K, A, K, B, K, pl.ACT_GELU))
+    s = torch.empty(n, device="cuda", dtype=torch.uint8)
+    lst = pl.TensorList([dA, dB, db])
+    ls = torch.empty(pl.tile_grad_norm_scratch_bytes(lst), device="cuda", dtype=torch.uint8)
+    norm = torch.zeros(1, device="cuda")
+    torch.cuda.synchronize()
+    def f():
+        kw = dict(scratch=s, scratch_bytes=n, stream=stream)
+        pl.tile_gemm_act(0, pl.BF16, "T", "N", M, N, K, 1.0, A, K, B, K, 0.0, None, M, D, M, act=pl.ACT_GELU, pre=P,
+                         ldPre=M, **kw)
+        pl.tile_gemm_act_grad(0, pl.BF16, "T", "N", M, N, K, 1.0, A, K, B, K, pl.ACT_GELU, P, M, D, M, dA=dA, lddA=K,
+                              dB=dB, lddB=K, dbias=db, **kw)
+        pl.tile_grad_clip(0, lst, 0.5, ls, norm=norm, stream=stream)
+    return f, (D, dA, dB, db, norm)
+
+st = torch.cuda.Stream()
+f, out = ops(st.cuda_stream, 515)
+# a first call inside a capture is refused and the capture goes on
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=st):
+    try:
+        f()
+        raise SystemExit("the first call was not refused")
+    except pl.ParaliaError as ex:
+        assert ex.code == pl.ERR_UNSUPPORTED, ex
+    out[0].add_(1)
+graph.replay()
+torch.cuda.synchronize()
+pl.fill_f32(torch.zeros(1, device="cuda"), 1, 0, 0, 0)
+# set up, but none of these kernels has run: their first launches are captured
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=st):
+    f()
+graph.replay()
+torch.cuda.synchronize()
+pl.tile_status(0)
+got = [t.clone() for t in out]
+f()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, out)) and float(out[4]) > 0
+# after a shutdown the library starts again
+pl.finalize()
+f()
+torch.cuda.synchronize()
+pl.tile_status(0)
+assert all(torch.equal(a, b) for a, b in zip(got, out))
+print("fresh ok")
+"""
+
+
+def test_first_calls_of_a_process():
+    """In a process of its own: a first call inside a capture, first launches inside a capture, and a shutdown."""
+    import subprocess
+    root = str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", FRESH, root], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0 and "fresh ok" in r.stdout, r.stdout + r.stderr
