@@ -333,7 +333,7 @@ int PARALiA_tile_ddot_noalloc(int dev, void* stream, int64_t N,
  * operands whose address and leading dimension are multiples of 16 bytes are read in place,
  * others are first copied to scratch. `scratch` is device memory on a 16-byte boundary of at least
  * PARALiA_tile_gemm_act_scratch_bytes(...) bytes (0 bytes: may be NULL). FP32 operands are
- * refused with PARALIA_ERR_UNSUPPORTED. */
+ * refused with PARALIA_ERR_UNSUPPORTED, and so are results of more than 2^30 - 128 rows or columns. */
 int64_t PARALiA_tile_gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N,
                                             int64_t K, const void* A, int64_t ldA, const void* B,
                                             int64_t ldB);

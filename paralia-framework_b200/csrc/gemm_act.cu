@@ -731,7 +731,10 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
         ga_prefetch_inputs<EW * 32>(a, QC ? q_first : r_first, QC ? q_cols : 128, QC ? r_first : q_first,
                                     QC ? 128 : q_cols);
       }
-      if (!mbar_wait_bounded(&ctl->acc_full[buf], (uint32_t)((local >> 1) & 1), abort_flag)) {
+      // every k block of the tile comes before it: 4096 clocks for each on top, three times what one
+      // takes where all SMs wait for HBM
+      if (!mbar_wait_bounded(&ctl->acc_full[buf], (uint32_t)((local >> 1) & 1), abort_flag,
+                             WAIT_BUDGET_CLOCKS + (long long)a.kblocks * 4096)) {
         if (!*abort_flag) { *abort_flag = 1; atomicExch(g.status, KERR_TMEM_WAIT_TIMEOUT); }
         ok = false;
         break;
@@ -1077,9 +1080,12 @@ double ga_cost(const GaPlan& v, const GemmActProblem* ps, int count) {
          (turns - 1.0) * 7.2 * (v.split > 1 ? 1.0 : 0.3) + (v.split > 1 ? 0.18 + 0.039 * v.split + 0.019 * v.bn : 0.0);
 }
 
-GaPlan ga_choose(const GemmActProblem* ps, int count, bool vec) {
-  GaPlan best{false, 16, 1, 1};
-  double best_cost = 1e300;
+struct GaChoice {
+  GaPlan plan;
+  double cost;
+};
+GaChoice ga_choose(const GemmActProblem* ps, int count, bool vec) {
+  GaChoice best{{false, 16, 1, 1}, 1e300};
   int64_t kb = INT32_MAX;
   for (int i = 0; i < count; ++i) kb = std::min(kb, std::max<int64_t>(1, ga_kblocks(ps[i].K)));
   for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
@@ -1087,10 +1093,7 @@ GaPlan ga_choose(const GemmActProblem* ps, int count, bool vec) {
       for (int split = 1; split <= (bn == 256 ? 1 : 8) && split <= kb; split *= 2) {
         const GaPlan v{qc != 0, bn, bn == 256 ? 2 : 1, split};
         const double c = ga_cost(v, ps, count);
-        if (c < best_cost) {
-          best_cost = c;
-          best = v;
-        }
+        if (c < best.cost) best = {v, c};
       }
     }
   }
@@ -1145,47 +1148,10 @@ int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int
   return ((rows + 7) / 8 * 8 * cols * 2 + 255) / 256 * 256;
 }
 
-int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream) {
-  GemmActProblem ps[GA_MAX_PROBS];
-  int n = 0;
-  for (int i = 0; i < count; ++i)
-    if (problems[i].M > 0 && problems[i].N > 0) ps[n++] = problems[i];
-  if (n == 0) return PARALIA_OK;
-  if (n == 2 && ps[1].K > ps[0].K && !ps[0].pre) std::swap(ps[0], ps[1]);
+namespace {
 
-  // operands that TMA cannot address where they are
-  AlignCopies copies;
-  memset(&copies, 0, sizeof(copies));
-  int copied = 0;
-  char* room = static_cast<char*>(scratch);
-  auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
-    const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
-    const int64_t ld8 = (rows + 7) / 8 * 8;
-    if (bytes > 0) {
-      copies.m[copied] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(room), ld, ld8, rows, cols};
-      copies.groups[copied++] = ld8 / 8 * cols;
-      q = room;
-      ld = ld8;
-      room += bytes;
-    } else if (cols <= 1) {
-      ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
-    }
-  };
-  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
-  bool vec = true;
-  for (int i = 0; i < n; ++i) {
-    GemmActProblem& p = ps[i];
-    vec = vec && vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) && vec16(p.bias, 0);
-    if (p.K == 0) continue;
-    in_reach(p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K);
-    in_reach(p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N);
-  }
-  if (copied > 0) {
-    const int64_t blocks = std::min<int64_t>((copies.groups[0] + copies.groups[1] + 255) / 256, GA_SMS * 16);
-    PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, copies));
-  }
-
-  const GaPlan v = ga_choose(ps, n, vec);
+// One launch of one or two products by plan v; their operands are where TMA can read them.
+int ga_launch_products(const GemmActProblem* ps, int n, const GaPlan& v, bool vec, int* status, cudaStream_t stream) {
   GaArgs g;
   GaMaps maps;
   memset(&g, 0, sizeof(g));
@@ -1207,9 +1173,6 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
     a.tile0 = (int32_t)tiles;
     const int64_t R = v.qc ? p.N : p.M, Q = v.qc ? p.M : p.N;
     const int64_t r_tiles = (R + 128 * v.cg - 1) / (128 * v.cg), q_tiles = (Q + v.bn - 1) / v.bn;
-    // the kernel numbers tiles, and panels of up to 16 of them, in 32 bits; clusters have up to 8 CTAs
-    if (r_tiles * std::max<int64_t>(q_tiles, 16) > INT32_MAX / 16 || tiles + r_tiles * q_tiles > INT32_MAX / 16)
-      return fail(PARALIA_ERR_UNSUPPORTED, "M = %d, N = %d: too many tiles", p.M, p.N);
     a.r_tiles = (int32_t)r_tiles;
     a.q_tiles = (int32_t)q_tiles;
     tiles += r_tiles * q_tiles;
@@ -1254,6 +1217,65 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
 #undef GA_CASE
   PL_CUDA(e);
   return PARALIA_OK;
+}
+
+}  // namespace
+
+int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream) {
+  GemmActProblem ps[GA_MAX_PROBS];
+  int n = 0;
+  for (int i = 0; i < count; ++i)
+    if (problems[i].M > 0 && problems[i].N > 0) ps[n++] = problems[i];
+  if (n == 0) return PARALIA_OK;
+  if (n == 2 && ps[1].K > ps[0].K && !ps[0].pre) std::swap(ps[0], ps[1]);
+
+  // operands that TMA cannot address where they are
+  AlignCopies copies;
+  memset(&copies, 0, sizeof(copies));
+  int copied = 0;
+  char* room = static_cast<char*>(scratch);
+  auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
+    const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
+    const int64_t ld8 = (rows + 7) / 8 * 8;
+    if (bytes > 0) {
+      copies.m[copied] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(room), ld, ld8, rows, cols};
+      copies.groups[copied++] = ld8 / 8 * cols;
+      q = room;
+      ld = ld8;
+      room += bytes;
+    } else if (cols <= 1) {
+      ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
+    }
+  };
+  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
+  bool vec = true;
+  for (int i = 0; i < n; ++i) {
+    GemmActProblem& p = ps[i];
+    vec = vec && vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) && vec16(p.bias, 0);
+    if (p.K == 0) continue;
+    in_reach(p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K);
+    in_reach(p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N);
+  }
+  if (copied > 0) {
+    const int64_t blocks = std::min<int64_t>((copies.groups[0] + copies.groups[1] + 255) / 256, GA_SMS * 16);
+    PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, copies));
+  }
+
+  // Two products go in one launch, which has one plan for both, or one after the other with a plan each:
+  // the gradient of a few columns is one product with hardly any k and many tiles and one with few tiles
+  // and much k, which alone is split. 6.2 us of estimate parts them best over 83 shapes: gradient of 16384 x
+  // 1 x 4096 222 us in one launch and 107 in two, 4096 x 64 x 1024 33 and 23, 4096 x 256 x 4096 44 and 51,
+  // 2999 x 1000 x 2048 58 and 78.
+  constexpr double second_launch = 6.2;
+  const GaChoice both = ga_choose(ps, n, vec);
+  if (n == 2) {
+    const GaChoice first = ga_choose(ps, 1, vec), second = ga_choose(ps + 1, 1, vec);
+    if (first.cost + second.cost + second_launch < both.cost) {
+      PL_TRY(ga_launch_products(ps, 1, first.plan, vec, status, stream));
+      return ga_launch_products(ps + 1, 1, second.plan, vec, status, stream);
+    }
+  }
+  return ga_launch_products(ps, n, both.plan, vec, status, stream);
 }
 
 cudaError_t launch_act_grad(const ActGradProblem& p, cudaStream_t stream) {

@@ -24,11 +24,15 @@ struct GemmActProblem {
   float alpha, beta;
 };
 
+// Rows and columns a result may have: tiles are numbered, with panels of up to 16 of them and clusters of
+// up to 8 CTAs, in 32 bits, and loops over rows or columns step past the end in them.
+constexpr int GA_MAX_ROWS = (1 << 30) - 128;
+
 // Bytes of the aligned copy that a stored rows x cols operand needs before TMA can read it; 0 if it
 // is read in place. A multiple of 256.
 int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols);
-// One or two products that do not depend on each other, of the same element type, in one launch; `pre`
-// only with the first. `scratch` (16-byte aligned) holds the copies of operands, at most two in all;
+// One or two products that do not depend on each other, of the same element type, in as few launches as
+// pay; `pre` only with the first. `scratch` (16-byte aligned) holds the copies of operands, at most two in all;
 // `status` is the GPU's word for waits that gave up. Returns a PARALIA_* code.
 int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream);
 

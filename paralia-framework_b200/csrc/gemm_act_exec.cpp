@@ -28,6 +28,9 @@ int check_common(int type, char TransA, char TransB, int64_t M, int64_t N, int64
   if (!is_flag(TransA) || !is_flag(TransB)) return fail(PARALIA_ERR_INVALID_ARG, "transpose flag is not N or T");
   if (M < 0 || N < 0 || K < 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
     return fail(PARALIA_ERR_INVALID_ARG, "dimension out of range");
+  if (M > GA_MAX_ROWS || N > GA_MAX_ROWS)
+    return fail(PARALIA_ERR_UNSUPPORTED, "M = %lld, N = %lld: more than %d rows or columns", (long long)M, (long long)N,
+                GA_MAX_ROWS);
   if (act < PARALIA_ACT_NONE || act > PARALIA_ACT_SILU)
     return fail(PARALIA_ERR_INVALID_ARG, "activation %d is not one of PARALIA_ACT_*", act);
   if (ldA < std::max<int64_t>(1, is_trans(TransA) ? K : M) || ldB < std::max<int64_t>(1, is_trans(TransB) ? N : K))
@@ -126,6 +129,8 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   PL_TRY(check_common(type, TransA, TransB, M, N, K, alpha, ldA, ldB, act));
   if (!std::isfinite(betaA) || !std::isfinite(betaB) || !std::isfinite(betaBias))
     return fail(PARALIA_ERR_INVALID_ARG, "beta is not finite");
+  if (K > GA_MAX_ROWS)
+    return fail(PARALIA_ERR_UNSUPPORTED, "K = %lld: more than %d rows or columns", (long long)K, GA_MAX_ROWS);
   const bool ta = is_trans(TransA), tb = is_trans(TransB);
   const bool uses_pre = act != PARALIA_ACT_NONE;
   const int64_t rows = std::max<int64_t>(1, M);

@@ -104,6 +104,12 @@ int check_max_norm(float max_norm) {
   return PARALIA_OK;
 }
 
+int check_results(const double* sumsq, const float* norm) {
+  if ((reinterpret_cast<uintptr_t>(sumsq) & 7) || (reinterpret_cast<uintptr_t>(norm) & 3))
+    return fail(PARALIA_ERR_INVALID_ARG, "sumsq or norm is not aligned to its type");
+  return PARALIA_OK;
+}
+
 int check_scratch(const void* scratch) {
   if (!scratch) return fail(PARALIA_ERR_INVALID_ARG, "NULL scratch");
   if (reinterpret_cast<uintptr_t>(scratch) & 7) return fail(PARALIA_ERR_INVALID_ARG, "scratch is not aligned to 8 bytes");
@@ -122,6 +128,7 @@ int exec_tile_grad_norm(int dev, void* stream, int count, const void* const* g, 
   GradList l;
   PL_TRY(describe(count, g, n, type, nullptr, nullptr, false, &entries, &l));
   PL_TRY(check_scratch(scratch));
+  PL_TRY(check_results(sumsq, norm));
   if (!sumsq && !norm) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq and norm");
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
@@ -140,6 +147,7 @@ int exec_tile_grad_clip(int dev, void* stream, int count, const void* const* g, 
   PL_TRY(check_max_norm(max_norm));
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   PL_TRY(check_scratch(scratch));
+  PL_TRY(check_results(sumsq, norm));
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -157,6 +165,7 @@ int exec_tile_grad_scale(int dev, void* stream, int count, const void* const* g,
   PL_TRY(check_max_norm(max_norm));
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   if (!sumsq) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq");
+  PL_TRY(check_results(sumsq, norm));
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
   // one partial sum is only read

@@ -268,6 +268,14 @@ def test_grad_whole_numbers_are_exact(pl, ta, tb, dims):
     _grad(pl, _defs(), "fp16", ta, tb, *dims, ints=True, act="relu")
 
 
+@pytest.mark.parametrize("ta,tb", TRANS)
+@pytest.mark.parametrize("pad,offset", [(0, 0), (3, 1)])
+@pytest.mark.parametrize("dims", [(4096, 8, 1024), (2050, 1, 4098), (4100, 100, 1100)])
+def test_grad_of_few_columns(pl, ta, tb, dims, pad, offset):
+    # one product with hardly any k, one with much: a launch each
+    _grad(pl, _defs(), "bf16", ta, tb, *dims, act="relu", betas=(1.0, 0.0, 0.0), pad=pad, offset=offset, ints=True)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("ta,tb", TRANS)

@@ -54,6 +54,14 @@ def test_grad_refusals(pl, kw):
     _refused(pl, _grad, **kw)
 
 
+def test_too_many_rows_or_columns_are_unsupported(pl):
+    n = (1 << 30) - 127
+    for kw in (dict(M=n, ldC=n, ldD=n), dict(N=n)):
+        _refused(pl, _call, code=pl.ERR_UNSUPPORTED, **kw)
+    for kw in (dict(M=n, ldPre=n, lddD=n), dict(N=n), dict(K=n, ldA=n, ldB=n, lddA=n, lddB=n)):
+        _refused(pl, _grad, code=pl.ERR_UNSUPPORTED, **kw)
+
+
 def test_what_is_empty_returns_at_once(pl):
     # nothing to compute: no GPU is asked for, no operand looked at
     _call(pl, M=0, A=0, D=0, Cm=0)
@@ -109,6 +117,15 @@ def test_list_refusals(pl):
         pl.tile_grad_norm(0, ok, S)                                   # nowhere to put the norm
     with pytest.raises(pl.ParaliaError):
         pl.tile_grad_norm(0, ok, 0, norm=D)
+    for kw in (dict(sumsq=D + 4), dict(norm=D + 2)):                  # results not aligned to their types
+        for f in (pl.tile_grad_norm, lambda *a, **k: pl.tile_grad_clip(*a[:2], 1.0, *a[2:], **k)):
+            with pytest.raises(pl.ParaliaError) as e:
+                f(0, ok, S, **kw)
+            assert e.value.code == pl.ERR_INVALID_ARG
+    for args, kw in (((D + 4, 1.0), {}), ((D, 1.0), dict(norm=D + 2))):
+        with pytest.raises(pl.ParaliaError) as e:
+            pl.tile_grad_scale(0, ok, *args, **kw)
+        assert e.value.code == pl.ERR_INVALID_ARG
 
 
 def test_tensor_list_checks(pl):
