@@ -330,9 +330,11 @@ int PARALiA_tile_ddot_noalloc(int dev, void* stream, int64_t N,
  * and weights w [out, in] is TransA = 'T', A = w, ldA = in, TransB = 'N', B = x, ldB = in,
  * M = out, N = tokens, K = in, D = y [tokens, out].
  * Any leading dimension and any address that is a multiple of the element size is accepted;
- * operands whose address and leading dimension are multiples of 16 bytes are read in place,
- * others are first copied to scratch. `scratch` is device memory on a 16-byte boundary of at least
- * PARALiA_tile_gemm_act_scratch_bytes(...) bytes (0 bytes: may be NULL). FP32 operands are
+ * operands whose address and leading dimension are multiples of 16 bytes can be read in place,
+ * others are first copied to scratch. `scratch` is device memory on a 16-byte boundary.
+ * PARALiA_tile_gemm_act_scratch_bytes(...) counts these copies and those that only make a large
+ * product faster (columns off 32-byte boundaries); given less, the call leaves the latter out and
+ * needs no scratch for operands on 16-byte boundaries. The result is the same. FP32 operands are
  * refused with PARALIA_ERR_UNSUPPORTED, and so are results of more than 2^30 - 128 rows or columns. */
 int64_t PARALiA_tile_gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N,
                                             int64_t K, const void* A, int64_t ldA, const void* B,

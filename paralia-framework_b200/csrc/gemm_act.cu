@@ -832,10 +832,11 @@ gemm_act_kernel(const __grid_constant__ GaMaps maps, const __grid_constant__ GaA
 
 // ------------------------------------------------------------------ copy to an aligned layout
 // A len x cols matrix at any 2-byte address and leading dimension, copied to a buffer whose columns
-// start on 16-byte boundaries, so that TMA can read it; up to two matrices in a launch. A thread
-// makes one aligned group of eight; in the middle of a column it takes the two aligned 16-byte
-// words that the group straddles and shifts them together, so both sides move at full width: 5003
-// columns of 1365 and 1237 of 1365 take 9 us from cold, a quarter of what the product after it takes.
+// start on 16-byte boundaries or better, so that TMA can read it, and fast; up to two matrices in a launch.
+// A thread makes one aligned group of eight from the two aligned 16-byte words that it straddles, shifted
+// together, so both sides move at full width. Bound by HBM: two matrices of 8192 x 8200 take 93 to 100 us, 5.6
+// TB/s; 5003 columns of 1365 and 1237 of 1365 take 10 from cold. Two groups of a thread in flight change
+// nothing, four take 105 us; columns worked on to the end of their padding cost a quarter more.
 struct AlignCopy {
   const uint16_t* src;
   uint16_t* dst;
@@ -854,14 +855,18 @@ __global__ void __launch_bounds__(256) align_copy_kernel(const __grid_constant__
     const bool second = i >= c.groups[0];
     const AlignCopy& m = c.m[second ? 1 : 0];
     const int64_t j = second ? i - c.groups[0] : i;
-    const int64_t groups = m.ld_dst >> 3;
-    const int64_t col = j / groups, g = j - col * groups;
-    const uint16_t* s = m.src + col * m.ld_src + g * 8;
+    const uint32_t groups = (uint32_t)((m.len + 7) >> 3);
+    const int64_t col = j < INT32_MAX ? (int64_t)((uint32_t)j / groups) : j / groups;
+    const int64_t at = (j - col * groups) * 8;
+    const uint16_t* s = m.src + col * m.ld_src + at;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(s) & 15) * 8;   // bits
+    // words inside the matrix; what they hold of a neighbouring column, or of the gap to it, ends up
+    // behind the copied column, where nobody reads
+    const int64_t left = col + 1 < m.cols ? m.ld_src + m.len - at : m.len - at;
     uint4 o;
-    if (g > 0 && g + 2 < groups) {
-      const int shift = (int)(reinterpret_cast<uintptr_t>(s) & 15) * 8;   // bits
+    if (shift == 0 ? left >= 8 : at + col * m.ld_src >= 8 && left >= 16) {
       const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(s) & ~uintptr_t(15));
-      const uint4 lo = p[0], hi = p[1];   // inside the column: one group of eight lies on either side
+      const uint4 lo = p[0], hi = shift == 0 ? lo : p[1];
       const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       const int word = shift >> 5, bits = shift & 31;
       uint32_t q[5];
@@ -873,9 +878,9 @@ __global__ void __launch_bounds__(256) align_copy_kernel(const __grid_constant__
       o.z = __funnelshift_r(q[2], q[3], bits);
       o.w = __funnelshift_r(q[3], q[4], bits);
     } else {
-      o = ga_load_any8(s, m.len - g * 8);
+      o = ga_load_any8(s, m.len - at);
     }
-    *reinterpret_cast<uint4*>(m.dst + col * m.ld_dst + g * 8) = o;
+    *reinterpret_cast<uint4*>(m.dst + col * m.ld_dst + at) = o;
   }
 }
 
@@ -1143,9 +1148,26 @@ bool ga_in_place(const void* p, int64_t ld, int64_t cols) {
 
 void gemm_act_forget_configuration() { ++ga_generation; }
 
-int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols) {
-  if (rows <= 0 || cols <= 0 || ga_in_place(p, ld, cols)) return 0;
-  return ((rows + 7) / 8 * 8 * cols * 2 + 255) / 256 * 256;
+int64_t gemm_act_copy_ld(int64_t rows) {
+  const int64_t q = rows < 64 ? 8 : rows < 512 ? 16 : 64;
+  return (rows + q - 1) / q * q;
+}
+
+int64_t gemm_act_copy_bytes(int64_t rows, int64_t cols) {
+  return (gemm_act_copy_ld(rows) * cols * 2 + 255) / 256 * 256;
+}
+
+// Columns that do not start on 32-byte sectors cost TMA five sectors and two lines for every 128 bytes:
+// 8192 x 8192 by k = 8200 takes 1161 us in place and 809 with copies (703 by k = 8192), 4096 x 4096 by 4104
+// 191 and 133, 8192 x 4096 by 1032 81 and 66; about 50 us for a GB that the SMs load. An element is
+// loaded once for 256 rows or columns of the result; the copy writes and reads it, 310 us for a GB, and
+// has to be waited for: small ones lose (4096 x 656 by 9320 53 us in place, 56 with B copied).
+GemmActCopy gemm_act_operand_copy(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t reuse) {
+  if (rows <= 0 || cols <= 0) return GA_COPY_NONE;
+  if (!ga_in_place(p, ld, cols)) return GA_COPY_NEEDED;
+  const bool sectors = (reinterpret_cast<uintptr_t>(p) & 31) == 0 && (cols <= 1 || (ld & 15) == 0);
+  const double gain = 50.0 * ((reuse + 255) / 256) - 310.0;   // us for a GB of operand
+  return !sectors && gain * (2e-9 * (double)rows * (double)cols) > 7.0 ? GA_COPY_PAYS : GA_COPY_NONE;
 }
 
 namespace {
@@ -1234,17 +1256,16 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
   memset(&copies, 0, sizeof(copies));
   int copied = 0;
   char* room = static_cast<char*>(scratch);
-  auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols) {
-    const int64_t bytes = gemm_act_operand_copy_bytes(q, ld, rows, cols);
-    const int64_t ld8 = (rows + 7) / 8 * 8;
-    if (bytes > 0) {
-      copies.m[copied] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(room), ld, ld8, rows, cols};
-      copies.groups[copied++] = ld8 / 8 * cols;
+  auto in_reach = [&](const void*& q, int64_t& ld, int64_t rows, int64_t cols, bool copy) {
+    const int64_t ld_copy = gemm_act_copy_ld(rows);
+    if (copy) {
+      copies.m[copied] = {static_cast<const uint16_t*>(q), reinterpret_cast<uint16_t*>(room), ld, ld_copy, rows, cols};
+      copies.groups[copied++] = (rows + 7) / 8 * cols;
       q = room;
-      ld = ld8;
-      room += bytes;
+      room += gemm_act_copy_bytes(rows, cols);
+      ld = ld_copy;
     } else if (cols <= 1) {
-      ld = ld8;   // of no meaning, but TMA wants a multiple of 16 bytes
+      ld = ld_copy;   // of no meaning, but TMA wants a multiple of 16 bytes
     }
   };
   auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
@@ -1253,11 +1274,11 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
     GemmActProblem& p = ps[i];
     vec = vec && vec16(p.D, p.ldD) && (!p.C || vec16(p.C, p.ldC)) && (!p.pre || vec16(p.pre, p.ldPre)) && vec16(p.bias, 0);
     if (p.K == 0) continue;
-    in_reach(p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K);
-    in_reach(p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N);
+    in_reach(p.A, p.ldA, p.ta ? p.K : p.M, p.ta ? p.M : p.K, p.copy_a != 0);
+    in_reach(p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N, p.copy_b != 0);
   }
   if (copied > 0) {
-    const int64_t blocks = std::min<int64_t>((copies.groups[0] + copies.groups[1] + 255) / 256, GA_SMS * 16);
+    const int64_t blocks = std::min<int64_t>((copies.groups[0] + copies.groups[1] + 255) / 256, GA_SMS * 32);
     PL_CUDA(launch_dependent(align_copy_kernel, (int)blocks, 256, 0, 1, stream, copies));
   }
 

@@ -19,6 +19,7 @@ struct GemmActProblem {
   int64_t ldA, ldB, ldC, ldD, ldPre;
   int32_t M, N, K;
   int32_t ta, tb;      // op is the transpose
+  int32_t copy_a, copy_b;   // the operand goes to scratch first, in an aligned layout
   int32_t act;         // PARALIA_ACT_*
   int32_t bf16;        // 1: BF16, 0: FP16
   float alpha, beta;
@@ -28,12 +29,17 @@ struct GemmActProblem {
 // up to 8 CTAs, in 32 bits, and loops over rows or columns step past the end in them.
 constexpr int GA_MAX_ROWS = (1 << 30) - 128;
 
-// Bytes of the aligned copy that a stored rows x cols operand needs before TMA can read it; 0 if it
-// is read in place. A multiple of 256.
-int64_t gemm_act_operand_copy_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols);
+// Leading dimension of an aligned copy of columns of `rows` elements: whole lines of 128 bytes unless
+// that were a large part of a column.
+int64_t gemm_act_copy_ld(int64_t rows);
+// The aligned copy of a stored rows x cols operand whose every element meets `reuse` rows or columns of
+// the result: whether TMA cannot read the operand without it, whether the product is faster with it.
+enum GemmActCopy : int { GA_COPY_NONE = 0, GA_COPY_PAYS = 1, GA_COPY_NEEDED = 2 };
+GemmActCopy gemm_act_operand_copy(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t reuse);
+int64_t gemm_act_copy_bytes(int64_t rows, int64_t cols);   // a multiple of 256
 // One or two products that do not depend on each other, of the same element type, in as few launches as
-// pay; `pre` only with the first. `scratch` (16-byte aligned) holds the copies of operands, at most two in all;
-// `status` is the GPU's word for waits that gave up. Returns a PARALIA_* code.
+// pay; `pre` only with the first. `scratch` (16-byte aligned) holds the copies of operands, at most two in all,
+// one behind the other; `status` is the GPU's word for waits that gave up. Returns a PARALIA_* code.
 int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, int* status, cudaStream_t stream);
 
 // Makes every GPU's kernels be configured anew at their next launch (library shutdown).

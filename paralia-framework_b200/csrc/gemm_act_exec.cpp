@@ -16,8 +16,6 @@ namespace {
 bool is_trans(char t) { return t == 'T' || t == 't' || t == 'C' || t == 'c'; }
 bool is_flag(char t) { return is_trans(t) || t == 'N' || t == 'n'; }
 
-int64_t round_up(int64_t v, int64_t q) { return (v + q - 1) / q * q; }
-
 // What the forward product and its gradient check alike.
 int check_common(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K, float alpha,
                  int64_t ldA, int64_t ldB, int act) {
@@ -52,13 +50,36 @@ bool odd_address(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) !=
 
 }  // namespace
 
+namespace {
+
+// What the operands of op(A) op(B) have in scratch: `bytes` with every copy that pays, `needed` with those
+// alone without which TMA cannot read an operand. The gradient reads A for N columns of dB and B
+// for M rows of dA, as the product itself does.
+struct OperandCopies {
+  GemmActCopy a, b;
+  int64_t bytes, needed;
+  // which copies are made with `room` bytes of scratch
+  bool make(GemmActCopy c, int64_t room) const { return c == GA_COPY_NEEDED || (c == GA_COPY_PAYS && room >= bytes); }
+};
+OperandCopies operand_copies(int64_t M, int64_t N, int64_t K, bool ta, bool tb, const void* A, int64_t ldA,
+                             const void* B, int64_t ldB) {
+  OperandCopies c;
+  const int64_t ra = ta ? K : M, ca = ta ? M : K, rb = tb ? N : K, cb = tb ? K : N;
+  c.a = gemm_act_operand_copy(A, ldA, ra, ca, N);
+  c.b = gemm_act_operand_copy(B, ldB, rb, cb, M);
+  const int64_t bytes_a = gemm_act_copy_bytes(ra, ca), bytes_b = gemm_act_copy_bytes(rb, cb);
+  c.bytes = (c.a != GA_COPY_NONE ? bytes_a : 0) + (c.b != GA_COPY_NONE ? bytes_b : 0);
+  c.needed = (c.a == GA_COPY_NEEDED ? bytes_a : 0) + (c.b == GA_COPY_NEEDED ? bytes_b : 0);
+  return c;
+}
+
+}  // namespace
+
 int64_t gemm_act_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
                                const void* A, int64_t ldA, const void* B, int64_t ldB) {
   if (check_common(type, TransA, TransB, M, N, K, 1.0f, ldA, ldB, PARALIA_ACT_NONE) != PARALIA_OK) return 0;
   if (M == 0 || N == 0 || K == 0) return 0;
-  const bool ta = is_trans(TransA), tb = is_trans(TransB);
-  return gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K) +
-         gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N);
+  return operand_copies(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB).bytes;
 }
 
 int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
@@ -78,8 +99,10 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   if (D == A || D == B || D == pre || D == bias || (pre && (pre == A || pre == B || pre == bias)) ||
       (beta != 0.0f && (pre == C || (D == C && ldD != ldC))))
     return fail(PARALIA_ERR_INVALID_ARG, "an output may share memory with no operand, but D with C at the same leading dimension");
-  const int64_t need = product ? gemm_act_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB) : 0;
-  if (need > 0) PL_TRY(check_scratch(scratch, scratch_bytes, need));
+  OperandCopies copies = {GA_COPY_NONE, GA_COPY_NONE, 0, 0};
+  if (product) copies = operand_copies(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB);
+  if (copies.needed > 0) PL_TRY(check_scratch(scratch, scratch_bytes, copies.needed));
+  const int64_t room = scratch && !(reinterpret_cast<uintptr_t>(scratch) & 15) ? scratch_bytes : 0;
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -90,6 +113,7 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   p.ldA = ldA; p.ldB = ldB; p.ldC = ldC; p.ldD = ldD; p.ldPre = ldPre;
   p.M = (int32_t)M; p.N = (int32_t)N; p.K = product ? (int32_t)K : 0;
   p.ta = is_trans(TransA); p.tb = is_trans(TransB);
+  p.copy_a = copies.make(copies.a, room); p.copy_b = copies.make(copies.b, room);
   p.act = act; p.bf16 = type == PARALIA_BF16;
   p.alpha = alpha; p.beta = beta;
   return launch_gemm_act(&p, 1, scratch, rt.dev(dev).status_dev, static_cast<cudaStream_t>(stream));
@@ -97,19 +121,18 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
 
 namespace {
 
-// Scratch of the gradient: dZ (M x N, leading dimension a multiple of eight; without an
-// activation the aligned copy of dD where it needs one), then the aligned copies of A and of B
-// where they need one.
+// Scratch of the gradient: dZ (M x N in an aligned layout; without an activation the copy of dD where it
+// has one), then the copies of A and of B.
 struct GradScratch {
-  int64_t ldZ, z_bytes, total;
+  int64_t ldZ, z_bytes;
+  OperandCopies copies;
 };
 GradScratch grad_scratch(int64_t M, int64_t N, int64_t K, bool ta, bool tb, const void* A, int64_t ldA, const void* B,
                          int64_t ldB) {
   GradScratch g;
-  g.ldZ = round_up(std::max<int64_t>(1, M), 8);
-  g.z_bytes = round_up(g.ldZ * N * 2, 256);
-  g.total = g.z_bytes + gemm_act_operand_copy_bytes(A, ldA, ta ? K : M, ta ? M : K) +
-            gemm_act_operand_copy_bytes(B, ldB, tb ? N : K, tb ? K : N);
+  g.ldZ = gemm_act_copy_ld(std::max<int64_t>(1, M));
+  g.z_bytes = gemm_act_copy_bytes(std::max<int64_t>(1, M), N);
+  g.copies = operand_copies(M, N, K, ta, tb, A, ldA, B, ldB);
   return g;
 }
 
@@ -118,7 +141,8 @@ GradScratch grad_scratch(int64_t M, int64_t N, int64_t K, bool ta, bool tb, cons
 int64_t gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M, int64_t N, int64_t K,
                                     const void* A, int64_t ldA, const void* B, int64_t ldB, int act) {
   if (check_common(type, TransA, TransB, M, N, K, 1.0f, ldA, ldB, act) != PARALIA_OK) return 0;
-  return grad_scratch(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB).total;
+  const GradScratch g = grad_scratch(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB);
+  return g.z_bytes + g.copies.bytes;
 }
 
 int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char TransB, int64_t M, int64_t N,
@@ -152,7 +176,7 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
       return fail(PARALIA_ERR_INVALID_ARG, "a gradient may share memory with no operand and no other gradient");
   }
   const GradScratch g = grad_scratch(M, N, K, ta, tb, A, ldA, B, ldB);
-  PL_TRY(check_scratch(scratch, scratch_bytes, g.total));
+  PL_TRY(check_scratch(scratch, scratch_bytes, g.z_bytes + g.copies.needed));
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -161,9 +185,9 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   const bool bf16 = type == PARALIA_BF16;
 
   // dZ and the bias gradient in one pass over dD and pre. Without an activation dZ is dD, in
-  // place if TMA can read it there.
+  // place unless it is to be copied.
   const bool products = entries && K > 0 && alpha != 0.0f && (want_a || want_b);
-  const bool need_z = products && (uses_pre || gemm_act_operand_copy_bytes(dD, lddD, M, N) > 0);
+  const bool need_z = products && (uses_pre || gemm_act_operand_copy(dD, lddD, M, N, K) != GA_COPY_NONE);
   char* base = static_cast<char*>(scratch);
   if (need_z || want_bias) {
     ActGradProblem a;
@@ -178,6 +202,9 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   void* copies = base + g.z_bytes;
   int* status = rt.dev(dev).status_dev;
 
+  const bool copy_a = g.copies.make(g.copies.a, scratch_bytes - g.z_bytes);
+  const bool copy_b = g.copies.make(g.copies.b, scratch_bytes - g.z_bytes);
+
   GemmActProblem ps[2];
   memset(ps, 0, sizeof(ps));
   int count = 0;
@@ -187,10 +214,10 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
     p.D = dB; p.ldD = lddB; p.C = betaB != 0.0f ? dB : nullptr; p.ldC = lddB; p.beta = betaB;
     p.K = alpha != 0.0f ? (int32_t)M : 0;
     if (!tb) {
-      p.A = A; p.ldA = ldA; p.ta = !ta; p.B = dZ; p.ldB = ldZ; p.tb = 0;
+      p.A = A; p.ldA = ldA; p.ta = !ta; p.copy_a = copy_a; p.B = dZ; p.ldB = ldZ; p.tb = 0;
       p.M = (int32_t)K; p.N = (int32_t)N;
     } else {
-      p.A = dZ; p.ldA = ldZ; p.ta = 1; p.B = A; p.ldB = ldA; p.tb = ta;
+      p.A = dZ; p.ldA = ldZ; p.ta = 1; p.B = A; p.ldB = ldA; p.tb = ta; p.copy_b = copy_a;
       p.M = (int32_t)N; p.N = (int32_t)K;
     }
   }
@@ -200,10 +227,10 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
     p.D = dA; p.ldD = lddA; p.C = betaA != 0.0f ? dA : nullptr; p.ldC = lddA; p.beta = betaA;
     p.K = alpha != 0.0f ? (int32_t)N : 0;
     if (!ta) {
-      p.A = dZ; p.ldA = ldZ; p.ta = 0; p.B = B; p.ldB = ldB; p.tb = !tb;
+      p.A = dZ; p.ldA = ldZ; p.ta = 0; p.B = B; p.ldB = ldB; p.tb = !tb; p.copy_b = copy_b;
       p.M = (int32_t)M; p.N = (int32_t)K;
     } else {
-      p.A = B; p.ldA = ldB; p.ta = tb; p.B = dZ; p.ldB = ldZ; p.tb = 1;
+      p.A = B; p.ldA = ldB; p.ta = tb; p.copy_a = copy_b; p.B = dZ; p.ldB = ldZ; p.tb = 1;
       p.M = (int32_t)K; p.N = (int32_t)M;
     }
   }

@@ -395,6 +395,29 @@ def test_offsets_beyond_32_bits(pl):
     assert torch.equal(D[:, rows], (B.float() @ A[rows].float().T).to(torch.bfloat16))
 
 
+@pytest.mark.parametrize("ta,tb", TRANS)
+def test_copies_that_pay(pl, ta, tb):
+    # columns between 32-byte sectors: copied where scratch is given, read in place where it is not; the same bits
+    import torch
+    M, N, K = 4104, 4120, 2056
+    g = torch.Generator(device="cuda").manual_seed(11)
+    (ra, ca), (rb, cb) = _stored(ta, M, K), _stored(tb, K, N)
+    A, B = (torch.randint(-2, 3, (c, r), generator=g, device="cuda").to(torch.bfloat16) for r, c in ((ra, ca), (rb, cb)))
+    n = pl.tile_gemm_act_scratch_bytes(pl.BF16, ta, tb, M, N, K, A, ra, B, rb)
+    assert n > 0
+    want = (B.T if tb == "T" else B).float() @ (A if ta == "N" else A.T).float()
+    out = []
+    for scratch, size in ((_scratch(n), n), (None, 0), (_scratch(64), 64)):
+        D = torch.zeros(N, M, dtype=torch.bfloat16, device="cuda")
+        pl.tile_gemm_act(0, pl.BF16, ta, tb, M, N, K, 1.0, A, ra, B, rb, 0.0, None, M, D, M, scratch=scratch,
+                         scratch_bytes=size)
+        out.append(D)
+    torch.cuda.synchronize()
+    pl.tile_status(0)
+    assert all(torch.equal(D, want.to(torch.bfloat16)) for D in out)
+    _grad(pl, _defs(), "bf16", ta, tb, M, N, K, act="none", alpha=0.5, ints=True)
+
+
 @pytest.mark.parametrize("N", [1, 40])
 def test_leading_dimensions_of_single_columns(pl, N):
     # a single column may have any leading dimension, a wide gap between columns is jumped over
