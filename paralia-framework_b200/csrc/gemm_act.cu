@@ -1044,44 +1044,37 @@ constexpr int GA_SMS = 148;
 
 std::atomic<unsigned> ga_generation{1};
 
-int64_t ga_tiles(const GaPlan& v, int64_t M, int64_t N) {
-  const int64_t R = v.qc ? N : M, Q = v.qc ? M : N;
-  return ((R + 128 * v.cg - 1) / (128 * v.cg)) * ((Q + v.bn - 1) / v.bn);
-}
-
 // Estimated microseconds of a variant (a constant common to all is left out). The constants are a fit
 // to 3100 timings of 134 shapes (1 to 2048 columns, 300 to 16384 rows, k 256 to 10240) with every
 // variant that fits them: the variant it picks is 1.2 % slower than the fastest in the mean, 30 % at
 // worst (1024 x 37 x 1024, 6.9 against 5.3 us).
-double ga_cost(const GaPlan& v, const GemmActProblem* ps, int count) {
-  int64_t tiles = 0, run = 0;
-  double hbm_bytes = 0.0, runs = 0.0;
+// Shifts and products in place of most divisions: this is host time of every call (forty variants, 0.22 us; 1.05 with them).
+double ga_cost(const GaPlan& v, const int64_t* tiles_of, const int64_t* kblocks, double hbm_bytes, int count) {
+  const int log_split = v.split == 1 ? 0 : v.split == 2 ? 1 : v.split == 4 ? 2 : 3;
+  int64_t tiles = 0, run = 0, run_sum = 0;
   for (int i = 0; i < count; ++i) {
-    const int64_t t = ga_tiles(v, ps[i].M, ps[i].N);
-    const int64_t r = (ga_kblocks(ps[i].K) + v.split - 1) / v.split;   // k blocks of a CTA
-    tiles += t;
-    runs += (double)t * r;
+    const int64_t r = (kblocks[i] + v.split - 1) >> log_split;   // k blocks of a CTA
+    tiles += tiles_of[i];
+    run_sum += tiles_of[i] * r;
     run = std::max(run, r);
-    hbm_bytes += 2.0 * ((double)ps[i].M * ps[i].K + (double)ps[i].K * ps[i].N + (double)ps[i].M * ps[i].N);
   }
-  const double mean_run = runs / tiles;
+  const double runs = (double)run_sum, mean_run = count == 1 ? (double)run : runs / (double)tiles;
   const int64_t ctas = tiles * v.cg * v.split;
-  const int per_sm = v.bn <= 64 ? 2 : 1;
   // CTAs an SM gets: clusters of 4 and 8 do not fill every group of SMs, 36 and 16 fit at a time
   const int64_t share = v.split == 1   ? (ctas + GA_SMS - 1) / GA_SMS
                         : v.split == 2 ? (tiles + 73) / 74
                         : v.split == 4 ? (tiles + 35) / 36
                                        : (tiles + 15) / 16;
-  const double turns = (double)((share + per_sm - 1) / per_sm);
+  const double turns = (double)(v.bn <= 64 ? (share + 1) >> 1 : share);   // two CTAs an SM, or one
   // a k block: MMAs at 1.4 times BN x 2 clocks, its bytes at 130 GB/s an SM, and 0.23 us from a CTA
   // that runs by itself
-  const double bytes = (128.0 + (double)v.bn / v.cg) * 128.0;
-  const double sm = std::max(mean_run * share, (double)run) * std::max(v.bn * 2 / 1900.0 * 1.4, bytes / 130e3);
+  const double bytes = (128.0 + (double)(v.cg == 2 ? v.bn / 2 : v.bn)) * 128.0;
+  const double sm = std::max(mean_run * (double)share, (double)run) * std::max(v.bn * (2 / 1900.0 * 1.4), bytes * (1 / 130e3));
   const double alone = std::max(mean_run * turns, (double)run) * 0.23;
-  const double in_flight = std::min(1.0, (double)ctas / (2 * GA_SMS));
-  const double hbm = hbm_bytes / 6.6e6 / (0.88 + 0.12 * in_flight);
-  const double l2 = runs * v.cg * v.split * bytes / 15e6;
-  return std::max(std::max(sm, alone), std::max(hbm, l2)) + 0.0079 * v.bn / v.split + (v.qc ? 0.0 : 0.017 * v.bn) +
+  const double in_flight = std::min(1.0, (double)ctas * (1.0 / (2 * GA_SMS)));
+  const double hbm = hbm_bytes * (1 / 6.6e6) / (0.88 + 0.12 * in_flight);
+  const double l2 = runs * (double)(v.cg * v.split) * bytes * (1 / 15e6);
+  return std::max(std::max(sm, alone), std::max(hbm, l2)) + (v.bn * 0.0079) / v.split + (v.qc ? 0.0 : 0.017 * v.bn) +
          (turns - 1.0) * 7.2 * (v.split > 1 ? 1.0 : 0.3) + (v.split > 1 ? 0.18 + 0.039 * v.split + 0.019 * v.bn : 0.0);
 }
 
@@ -1091,13 +1084,24 @@ struct GaChoice {
 };
 GaChoice ga_choose(const GemmActProblem* ps, int count, bool vec) {
   GaChoice best{{false, 16, 1, 1}, 1e300};
-  int64_t kb = INT32_MAX;
-  for (int i = 0; i < count; ++i) kb = std::min(kb, std::max<int64_t>(1, ga_kblocks(ps[i].K)));
+  int64_t kb = INT32_MAX, kblocks[GA_MAX_PROBS], tiles[GA_MAX_PROBS];
+  double hbm_bytes = 0.0;
+  for (int i = 0; i < count; ++i) {
+    const double M = ps[i].M, N = ps[i].N, K = ps[i].K;
+    kblocks[i] = ga_kblocks(ps[i].K);
+    kb = std::min(kb, std::max<int64_t>(1, kblocks[i]));
+    hbm_bytes += 2.0 * (M * K + K * N + M * N);
+  }
   for (int qc = vec ? 1 : 0; qc >= 0; --qc) {
     for (int bn = qc ? 64 : 16; bn <= 256; bn = bn < 64 ? bn + 16 : bn * 2) {
+      const int cg = bn == 256 ? 2 : 1;
+      for (int i = 0; i < count; ++i) {
+        const uint32_t R = (uint32_t)(qc ? ps[i].N : ps[i].M), Q = (uint32_t)(qc ? ps[i].M : ps[i].N);
+        tiles[i] = (int64_t)((R + 128 * cg - 1) >> (cg == 2 ? 8 : 7)) * ((Q + bn - 1) / (uint32_t)bn);
+      }
       for (int split = 1; split <= (bn == 256 ? 1 : 8) && split <= kb; split *= 2) {
-        const GaPlan v{qc != 0, bn, bn == 256 ? 2 : 1, split};
-        const double c = ga_cost(v, ps, count);
+        const GaPlan v{qc != 0, bn, cg, split};
+        const double c = ga_cost(v, tiles, kblocks, hbm_bytes, count);
         if (c < best.cost) best = {v, c};
       }
     }
