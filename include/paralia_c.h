@@ -357,7 +357,9 @@ int PARALiA_tile_gemm_act(int dev, void* stream, int type, char TransA, char Tra
  * beta of 1 adds to what earlier calls left (shared weights, several micro-batches). dZ is
  * rounded to `type` before the two products, which take 16-bit operands; dbias is summed in
  * FP32 from the unrounded dZ. No gradient may share memory with another or with an operand.
- * `scratch`: PARALiA_tile_gemm_act_grad_scratch_bytes(...) bytes on a 16-byte boundary. */
+ * `scratch`: PARALiA_tile_gemm_act_grad_scratch_bytes(...) bytes on a 16-byte boundary. That counts room
+ * for dZ; a call that makes none (PARALIA_ACT_NONE with dD on 16-byte boundaries, no columns, alpha 0,
+ * dbias alone) takes less, and NULL if nothing is left. */
 int64_t PARALiA_tile_gemm_act_grad_scratch_bytes(int type, char TransA, char TransB, int64_t M,
                                                  int64_t N, int64_t K, const void* A, int64_t ldA,
                                                  const void* B, int64_t ldB, int act);

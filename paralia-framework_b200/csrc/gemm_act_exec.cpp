@@ -175,8 +175,15 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
     if (outs[i] == A || outs[i] == B || outs[i] == pre || outs[i] == dD || outs[i] == outs[(i + 1) % 3])
       return fail(PARALIA_ERR_INVALID_ARG, "a gradient may share memory with no operand and no other gradient");
   }
+  // What this call touches of its scratch: nothing without a product; without an activation dZ is dD, in
+  // place unless it is to be copied.
   const GradScratch g = grad_scratch(M, N, K, ta, tb, A, ldA, B, ldB);
-  PL_TRY(check_scratch(scratch, scratch_bytes, g.z_bytes + g.copies.needed));
+  const bool products = entries && K > 0 && alpha != 0.0f && (want_a || want_b);
+  const int64_t room = scratch && !(reinterpret_cast<uintptr_t>(scratch) & 15) ? scratch_bytes : 0;
+  const GemmActCopy copy_z = uses_pre ? GA_COPY_NEEDED : gemm_act_operand_copy(dD, lddD, M, N, K);
+  const bool need_z = products && (copy_z == GA_COPY_NEEDED || (copy_z == GA_COPY_PAYS && room >= g.z_bytes + g.copies.needed));
+  const int64_t z_bytes = need_z ? g.z_bytes : 0, needed = products ? z_bytes + g.copies.needed : 0;
+  if (needed > 0) PL_TRY(check_scratch(scratch, scratch_bytes, needed));
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -184,10 +191,7 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = type == PARALIA_BF16;
 
-  // dZ and the bias gradient in one pass over dD and pre. Without an activation dZ is dD, in
-  // place unless it is to be copied.
-  const bool products = entries && K > 0 && alpha != 0.0f && (want_a || want_b);
-  const bool need_z = products && (uses_pre || gemm_act_operand_copy(dD, lddD, M, N, K) != GA_COPY_NONE);
+  // dZ and the bias gradient in one pass over dD and pre
   char* base = static_cast<char*>(scratch);
   if (need_z || want_bias) {
     ActGradProblem a;
@@ -199,11 +203,11 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   }
   const void* dZ = need_z ? base : dD;
   const int64_t ldZ = need_z ? g.ldZ : lddD;
-  void* copies = base + g.z_bytes;
+  void* copies = base + z_bytes;
   int* status = rt.dev(dev).status_dev;
 
-  const bool copy_a = g.copies.make(g.copies.a, scratch_bytes - g.z_bytes);
-  const bool copy_b = g.copies.make(g.copies.b, scratch_bytes - g.z_bytes);
+  const bool copy_a = g.copies.make(g.copies.a, room - z_bytes);
+  const bool copy_b = g.copies.make(g.copies.b, room - z_bytes);
 
   GemmActProblem ps[2];
   memset(ps, 0, sizeof(ps));
