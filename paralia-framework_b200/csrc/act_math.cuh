@@ -68,8 +68,10 @@ __device__ __forceinline__ float normal_tail(float x) {
   return t * exp2_f32(fmaf(-w, w, p));
 }
 
-// The three smooth activations vanish to the left faster than any 16-bit type resolves, so z
-// is clamped there: act(-inf) is then 0 and not inf * 0. A NaN stays a NaN throughout.
+// The sigmoid, or the tail probability, is 0 from where it falls below 2^-126. z is clamped to the left of
+// that place, where it is 0 already: act(-inf) is then 0 and not inf * 0. What a finite z loses is below
+// |z| * 2^-126 at the place itself, 1e-36 at most (BF16 has numbers down to there, so nothing nearer
+// will do as a clamp: silu(-85) is -1e-35). A NaN stays a NaN throughout.
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
   if (ACT == PARALIA_ACT_RELU) return z < 0.0f ? 0.0f : z;
@@ -79,11 +81,11 @@ __device__ __forceinline__ float act_value(float z) {
   }
   if (ACT == PARALIA_ACT_GELU_TANH) {
     constexpr float K1 = -2.0f * GELU_C * LOG2E, K2 = K1 * GELU_A;
-    const float c = max_nan(z, -9.0f);    // the exponent is 95 there
+    const float c = max_nan(z, -10.2f);   // the exponent is 132 there
     return c * sigmoid_exp2(c * fmaf(K2, c * c, K1));
   }
   if (ACT == PARALIA_ACT_SILU) {
-    const float c = max_nan(z, -80.0f);
+    const float c = max_nan(z, -90.0f);   // the exponent is 129 there
     return c * sigmoid_exp2(-LOG2E * c);
   }
   return z;
@@ -100,12 +102,12 @@ __device__ __forceinline__ float act_slope(float z) {
   }
   if (ACT == PARALIA_ACT_GELU_TANH) {
     constexpr float K1 = -2.0f * GELU_C * LOG2E, K2 = K1 * GELU_A;
-    const float c = min_nan(max_nan(z, -9.0f), 9.0f), q = c * c;
+    const float c = min_nan(max_nan(z, -10.2f), 10.2f), q = c * c;
     const float g = sigmoid_exp2(c * fmaf(K2, q, K1));
     return fmaf(c * fmaf(6.0f * GELU_C * GELU_A, q, 2.0f * GELU_C), g * (1.0f - g), g);
   }
   if (ACT == PARALIA_ACT_SILU) {
-    const float c = min_nan(max_nan(z, -80.0f), 80.0f);
+    const float c = min_nan(max_nan(z, -90.0f), 90.0f);
     const float g = sigmoid_exp2(-LOG2E * c);
     return fmaf(c * g, 1.0f - g, g);
   }
