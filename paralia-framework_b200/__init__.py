@@ -243,12 +243,16 @@ def _ptr(x) -> int:
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 
-def _dev_ptr(x) -> int:
-    """Address of an operand of the mixed-precision routines, which take GPU memory only."""
+def _dev_ptr(x, dev=None) -> int:
+    """Address of an operand of the mixed-precision routines, which take memory of GPU ``dev`` only (None: of any GPU)."""
     if x is None or isinstance(x, int):
         return x or 0
-    if not getattr(x, "is_cuda", False):
+    get_device = getattr(x, "get_device", None)
+    at = -1 if get_device is None else get_device()
+    if at < 0:
         raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
+    if at != dev and dev is not None:
+        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is on GPU {at}, the call is for GPU {dev}")
     return x.data_ptr()
 
 
@@ -459,9 +463,10 @@ def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, bet
                   scratch_bytes: int = 0, stream: int = 0) -> None:
     """``Z = alpha*op(A)*op(B) + bias``, ``pre <- Z``, ``D <- act(Z) + beta*Cm``, FP16 or BF16 (``type``),
     column-major, on the caller's stream. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A), ldA,
-                                       _dev_ptr(B), ldB, _dev_ptr(bias), act, beta, _dev_ptr(Cm), ldC, _dev_ptr(D), ldD,
-                                       _dev_ptr(pre), ldPre, _dev_ptr(scratch), scratch_bytes))
+    _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A, dev), ldA,
+                                       _dev_ptr(B, dev), ldB, _dev_ptr(bias, dev), act, beta, _dev_ptr(Cm, dev), ldC,
+                                       _dev_ptr(D, dev), ldD, _dev_ptr(pre, dev), ldPre, _dev_ptr(scratch, dev),
+                                       scratch_bytes))
 
 
 def tile_gemm_act_grad_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB, act) -> int:
@@ -475,10 +480,10 @@ def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB
                        stream: int = 0) -> None:
     """Gradient of ``tile_gemm_act``: ``dA``, ``dB`` and ``dbias`` (each may be None) from the gradient ``dD``
     of its result and the pre-activation ``pre`` it kept. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A),
-                                            ldA, _dev_ptr(B), ldB, act, _dev_ptr(pre), ldPre, _dev_ptr(dD), lddD, betaA,
-                                            _dev_ptr(dA), lddA, betaB, _dev_ptr(dB), lddB, betaBias, _dev_ptr(dbias),
-                                            _dev_ptr(scratch), scratch_bytes))
+    _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A, dev),
+                                            ldA, _dev_ptr(B, dev), ldB, act, _dev_ptr(pre, dev), ldPre, _dev_ptr(dD, dev),
+                                            lddD, betaA, _dev_ptr(dA, dev), lddA, betaB, _dev_ptr(dB, dev), lddB,
+                                            betaBias, _dev_ptr(dbias, dev), _dev_ptr(scratch, dev), scratch_bytes))
 
 
 _TYPE_OF = {"float32": F32, "float16": F16, "bfloat16": BF16}
@@ -499,6 +504,7 @@ class TensorList:
     def __init__(self, tensors, out=None):
         self.tensors = list(tensors)
         self.out = None if out is None else list(out)
+        self.dev = None         # the GPU that holds them
         if self.out is not None and len(self.out) != len(self.tensors):
             raise ParaliaError(ERR_INVALID_ARG, f"{len(self.tensors)} tensors, {len(self.out)} outputs")
         for i, t in enumerate(self.tensors):
@@ -508,6 +514,10 @@ class TensorList:
                     raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} is not contiguous")
                 if getattr(x, "is_cuda", True) is False:
                     raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} is not in GPU memory")
+                at = x.get_device() if hasattr(x, "get_device") else self.dev
+                if self.dev is not None and at != self.dev:
+                    raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} is on GPU {at}, those before it on GPU {self.dev}")
+                self.dev = at
             if o.numel() != t.numel():
                 raise ParaliaError(ERR_INVALID_ARG, f"tensor {i} has {t.numel()} elements, its output {o.numel()}")
         n = self.count = len(self.tensors)
@@ -518,6 +528,12 @@ class TensorList:
         self.out_type = None if self.out is None else (_i32 * n)(*[_type_of(t) for t in self.out])
 
 
+def _list_on(grads, dev) -> None:
+    at = getattr(grads, "dev", None)
+    if at != dev and at is not None:
+        raise ParaliaError(ERR_INVALID_ARG, f"the list is on GPU {at}, the call is for GPU {dev}")
+
+
 def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
     return int(lib().PARALiA_tile_grad_norm_scratch_bytes(grads.count))
 
@@ -525,22 +541,26 @@ def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
 def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of a list of tensors: ``norm`` (float32) and ``sumsq`` (float64, its square) are device
     scalars, either may be None. No counterpart in the reference."""
-    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _dev_ptr(scratch),
-                                        _dev_ptr(sumsq), _dev_ptr(norm)))
+    _list_on(grads, dev)
+    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _dev_ptr(scratch, dev),
+                                        _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
 
 
 def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of the list, then every tensor times ``max_norm / norm`` where that is below 1, in place or
     to the list's ``out``. No counterpart in the reference."""
+    _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                        grads.out_type, max_norm, _dev_ptr(scratch), _dev_ptr(sumsq), _dev_ptr(norm)))
+                                        grads.out_type, max_norm, _dev_ptr(scratch, dev), _dev_ptr(sumsq, dev),
+                                        _dev_ptr(norm, dev)))
 
 
 def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:
     """The scaling half of ``tile_grad_clip`` from a squared norm in device memory (the sum over several
     GPUs' lists). No counterpart in the reference."""
+    _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_scale(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                         grads.out_type, _dev_ptr(sumsq), max_norm, _dev_ptr(norm)))
+                                         grads.out_type, _dev_ptr(sumsq, dev), max_norm, _dev_ptr(norm, dev)))
 
 
 def malloc(nbytes: int, loc: int) -> int:

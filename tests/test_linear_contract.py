@@ -19,7 +19,7 @@ def _grad(pl, **kw):
 
 def _passes(text):
     """Whether a call came as far as its GPU: there is none, or not so many."""
-    return "no CUDA device" in text or "out of range" in text
+    return "no CUDA device" in text or f"GPU id {NO_GPU}" in text
 
 
 def test_gradient_asks_for_no_scratch_that_it_does_not_touch(pl):
@@ -31,3 +31,70 @@ def test_gradient_asks_for_no_scratch_that_it_does_not_touch(pl):
     assert _passes(_grad(pl, alpha=0.0, **none))
     assert "bytes of scratch" in _grad(pl, act=pl.ACT_NONE, dD=D + 2, **none)       # dD has to be copied
     assert "bytes of scratch" in _grad(pl, act=pl.ACT_NONE, A=A + 2, **none)
+
+
+class Tensor:
+    """Looks like a GPU tensor at `address`."""
+
+    def __init__(self, address, gpu=0, dtype="torch.uint8", numel=1 << 12, element_size=1):
+        self.address, self.gpu, self.dtype, self.n, self.size, self.is_cuda = address, gpu, dtype, numel, element_size, True
+
+    def data_ptr(self):
+        return self.address
+
+    def get_device(self):
+        return self.gpu
+
+    def numel(self):
+        return self.n
+
+    def element_size(self):
+        return self.size
+
+    def is_contiguous(self):
+        return True
+
+
+def _forward(pl, **kw):
+    a = dict(dev=NO_GPU, type=pl.BF16, TransA="T", TransB="N", M=64, N=32, K=16, alpha=1.0, A=A, ldA=16, B=B, ldB=16,
+             beta=1.0, Cm=CC, ldC=64, D=D, ldD=64, bias=DBIAS, pre=P, ldPre=64, scratch=S, scratch_bytes=4096)
+    a.update(kw)
+    with pytest.raises(pl.ParaliaError) as e:
+        pl.tile_gemm_act(**a)
+    return str(e.value)
+
+
+def _lists(pl, lst, dev=NO_GPU, scratch=S, sumsq=D, norm=P):
+    """What the three list routines say."""
+    out = []
+    for f in (lambda: pl.tile_grad_norm(dev, lst, scratch, norm=norm, sumsq=sumsq),
+              lambda: pl.tile_grad_clip(dev, lst, 1.0, scratch, norm=norm, sumsq=sumsq),
+              lambda: pl.tile_grad_scale(dev, lst, sumsq, 1.0, norm=norm)):
+        with pytest.raises(pl.ParaliaError) as e:
+            f()
+        out.append(str(e.value))
+    return out
+
+
+def test_tensors_of_another_gpu_are_refused(pl):
+    here, other = Tensor(A, NO_GPU), Tensor(A, 1)
+    assert _passes(_forward(pl)) and _passes(_grad(pl))
+    for name in ("A", "B", "Cm", "D", "bias", "pre", "scratch"):
+        at = {"A": A, "B": B, "Cm": CC, "D": D, "bias": DBIAS, "pre": P, "scratch": S}[name]
+        assert _passes(_forward(pl, **{name: Tensor(at, NO_GPU)})), name
+        assert "is on GPU 1" in _forward(pl, **{name: Tensor(at, 1)}), name
+    for name in ("A", "B", "pre", "dD", "dA", "dB", "dbias", "scratch"):
+        assert "is on GPU 1" in _grad(pl, **{name: other}), name
+    f32 = lambda address, gpu: Tensor(address, gpu, "torch.float32", 64, 4)
+    lst = pl.TensorList([f32(A, 1), f32(B, 1)])
+    assert all("is on GPU 1" in t for t in _lists(pl, lst))
+    lst = pl.TensorList([f32(A, NO_GPU)], [f32(B, NO_GPU)])
+    assert all(_passes(t) for t in _lists(pl, lst))
+    f64 = Tensor(D, 1, "torch.float64", 1, 8)
+    assert all("is on GPU 1" in t for t in _lists(pl, lst, sumsq=f64))
+    assert all("is on GPU 1" in t for t in _lists(pl, lst, norm=f32(P, 1)))
+    assert all("is on GPU 1" in t for t in _lists(pl, lst, scratch=Tensor(S, 1))[:2])
+    for lists in (([f32(A, 0), f32(B, 1)],), ([f32(A, 0)], [f32(B, 1)])):
+        with pytest.raises(pl.ParaliaError):
+            pl.TensorList(*lists)
+    assert _passes(_forward(pl, A=here))
