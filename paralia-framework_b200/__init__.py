@@ -256,6 +256,14 @@ def _dev_ptr(x, dev=None) -> int:
     return x.data_ptr()
 
 
+def _scratch_ptr(x, nbytes, dev) -> int:
+    """Address of scratch of which a call may use ``nbytes``; a tensor has to hold as many."""
+    at = _dev_ptr(x, dev)
+    if at and not isinstance(x, int) and x.nbytes < nbytes:
+        raise ParaliaError(ERR_INVALID_ARG, f"scratch holds {x.nbytes} bytes, {nbytes} are to be used")
+    return at
+
+
 _FLAGS = {ch: ch.encode() for ch in "NTCntc"}
 
 
@@ -465,7 +473,7 @@ def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, bet
     column-major, on the caller's stream. No counterpart in the reference."""
     _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A, dev), ldA,
                                        _dev_ptr(B, dev), ldB, _dev_ptr(bias, dev), act, beta, _dev_ptr(Cm, dev), ldC,
-                                       _dev_ptr(D, dev), ldD, _dev_ptr(pre, dev), ldPre, _dev_ptr(scratch, dev),
+                                       _dev_ptr(D, dev), ldD, _dev_ptr(pre, dev), ldPre, _scratch_ptr(scratch, scratch_bytes, dev),
                                        scratch_bytes))
 
 
@@ -483,7 +491,8 @@ def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB
     _check(lib().PARALiA_tile_gemm_act_grad(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A, dev),
                                             ldA, _dev_ptr(B, dev), ldB, act, _dev_ptr(pre, dev), ldPre, _dev_ptr(dD, dev),
                                             lddD, betaA, _dev_ptr(dA, dev), lddA, betaB, _dev_ptr(dB, dev), lddB,
-                                            betaBias, _dev_ptr(dbias, dev), _dev_ptr(scratch, dev), scratch_bytes))
+                                            betaBias, _dev_ptr(dbias, dev), _scratch_ptr(scratch, scratch_bytes, dev),
+                                            scratch_bytes))
 
 
 _TYPE_OF = {"float32": F32, "float16": F16, "bfloat16": BF16}
@@ -505,6 +514,7 @@ class TensorList:
         self.tensors = list(tensors)
         self.out = None if out is None else list(out)
         self.dev = None         # the GPU that holds them
+        self.scratch_bytes = None   # that the norm needs, once it has been asked for
         if self.out is not None and len(self.out) != len(self.tensors):
             raise ParaliaError(ERR_INVALID_ARG, f"{len(self.tensors)} tensors, {len(self.out)} outputs")
         for i, t in enumerate(self.tensors):
@@ -534,6 +544,14 @@ def _list_on(grads, dev) -> None:
         raise ParaliaError(ERR_INVALID_ARG, f"the list is on GPU {at}, the call is for GPU {dev}")
 
 
+def _list_scratch(grads, scratch, dev) -> int:
+    if scratch is None or isinstance(scratch, int):
+        return scratch or 0
+    if grads.scratch_bytes is None:
+        grads.scratch_bytes = tile_grad_norm_scratch_bytes(grads)
+    return _scratch_ptr(scratch, grads.scratch_bytes, dev)
+
+
 def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
     return int(lib().PARALiA_tile_grad_norm_scratch_bytes(grads.count))
 
@@ -542,8 +560,8 @@ def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, strea
     """Global norm of a list of tensors: ``norm`` (float32) and ``sumsq`` (float64, its square) are device
     scalars, either may be None. No counterpart in the reference."""
     _list_on(grads, dev)
-    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type, _dev_ptr(scratch, dev),
-                                        _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
+    _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type,
+                                        _list_scratch(grads, scratch, dev), _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
 
 
 def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
@@ -551,8 +569,8 @@ def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=N
     to the list's ``out``. No counterpart in the reference."""
     _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                        grads.out_type, max_norm, _dev_ptr(scratch, dev), _dev_ptr(sumsq, dev),
-                                        _dev_ptr(norm, dev)))
+                                        grads.out_type, max_norm, _list_scratch(grads, scratch, dev),
+                                        _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
 
 
 def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:

@@ -51,6 +51,10 @@ class Tensor:
     def element_size(self):
         return self.size
 
+    @property
+    def nbytes(self):
+        return self.n * self.size
+
     def is_contiguous(self):
         return True
 
@@ -98,3 +102,16 @@ def test_tensors_of_another_gpu_are_refused(pl):
         with pytest.raises(pl.ParaliaError):
             pl.TensorList(*lists)
     assert _passes(_forward(pl, A=here))
+
+
+def test_scratch_smaller_than_said_is_refused(pl):
+    scratch = lambda numel, size=1: Tensor(S, NO_GPU, "torch.uint8", numel, size)
+    for f in (_forward, _grad):
+        assert _passes(f(pl, scratch=scratch(4096), scratch_bytes=4096))
+        assert _passes(f(pl, scratch=scratch(1024, 4), scratch_bytes=4096))
+        assert "scratch holds 4095 bytes" in f(pl, scratch=scratch(4095), scratch_bytes=4096)
+    lst = pl.TensorList([Tensor(A, NO_GPU, "torch.float32", 64, 4)])
+    n = pl.tile_grad_norm_scratch_bytes(lst)
+    assert all(_passes(t) for t in _lists(pl, lst, scratch=scratch(n)))
+    norm, clip, scale = _lists(pl, lst, scratch=scratch(n - 8))
+    assert "scratch holds" in norm and "scratch holds" in clip and _passes(scale)
