@@ -247,19 +247,24 @@ def _dev_ptr(x, dev=None) -> int:
     """Address of an operand of the mixed-precision routines, which take memory of GPU ``dev`` only (None: of any GPU)."""
     if x is None or isinstance(x, int):
         return x or 0
-    get_device = getattr(x, "get_device", None)
-    at = -1 if get_device is None else get_device()
-    if at < 0:
-        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
-    if at != dev and dev is not None:
-        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is on GPU {at}, the call is for GPU {dev}")
+    try:
+        at = x.get_device()
+    except AttributeError:
+        at = -1
+    if at != dev or at < 0:
+        if at < 0:
+            raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
+        if dev is not None:
+            raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is on GPU {at}, the call is for GPU {dev}")
     return x.data_ptr()
 
 
 def _scratch_ptr(x, nbytes, dev) -> int:
     """Address of scratch of which a call may use ``nbytes``; a tensor has to hold as many."""
+    if x is None or isinstance(x, int):
+        return x or 0
     at = _dev_ptr(x, dev)
-    if at and not isinstance(x, int) and x.nbytes < nbytes:
+    if x.nbytes < nbytes:
         raise ParaliaError(ERR_INVALID_ARG, f"scratch holds {x.nbytes} bytes, {nbytes} are to be used")
     return at
 
@@ -473,8 +478,8 @@ def tile_gemm_act(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB, bet
     column-major, on the caller's stream. No counterpart in the reference."""
     _check(lib().PARALiA_tile_gemm_act(dev, stream, type, _c(TransA), _c(TransB), M, N, K, alpha, _dev_ptr(A, dev), ldA,
                                        _dev_ptr(B, dev), ldB, _dev_ptr(bias, dev), act, beta, _dev_ptr(Cm, dev), ldC,
-                                       _dev_ptr(D, dev), ldD, _dev_ptr(pre, dev), ldPre, _scratch_ptr(scratch, scratch_bytes, dev),
-                                       scratch_bytes))
+                                       _dev_ptr(D, dev), ldD, _dev_ptr(pre, dev), ldPre,
+                                       _scratch_ptr(scratch, scratch_bytes, dev), scratch_bytes))
 
 
 def tile_gemm_act_grad_scratch_bytes(type, TransA, TransB, M, N, K, A, ldA, B, ldB, act) -> int:
@@ -495,11 +500,31 @@ def tile_gemm_act_grad(dev, type, TransA, TransB, M, N, K, alpha, A, ldA, B, ldB
                                             scratch_bytes))
 
 
+_DTYPE_NAMES = {}
+
+
+def _dtype_name(x) -> str:
+    name = _DTYPE_NAMES.get(x.dtype)
+    if name is None:
+        name = _DTYPE_NAMES[x.dtype] = str(x.dtype).rsplit(".", 1)[-1]
+    return name
+
+
+def _scalar_ptr(x, dtype: str, dev) -> int:
+    """Address of a device scalar that a list routine reads or writes as ``dtype``."""
+    if x is None or isinstance(x, int):
+        return x or 0
+    at = _dev_ptr(x, dev)
+    if _dtype_name(x) != dtype or x.nbytes == 0:
+        raise ParaliaError(ERR_INVALID_ARG, f"{x.nbytes} bytes of {_dtype_name(x)} where a {dtype} is read or written")
+    return at
+
+
 _TYPE_OF = {"float32": F32, "float16": F16, "bfloat16": BF16}
 
 
 def _type_of(x) -> int:
-    name = str(x.dtype).rsplit(".", 1)[-1]
+    name = _dtype_name(x)
     if name not in _TYPE_OF:
         raise ParaliaError(ERR_INVALID_ARG, f"element type {name} is not float32, float16 or bfloat16")
     return _TYPE_OF[name]
@@ -561,7 +586,8 @@ def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, strea
     scalars, either may be None. No counterpart in the reference."""
     _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type,
-                                        _list_scratch(grads, scratch, dev), _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
+                                        _list_scratch(grads, scratch, dev), _scalar_ptr(sumsq, "float64", dev),
+                                        _scalar_ptr(norm, "float32", dev)))
 
 
 def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
@@ -570,7 +596,7 @@ def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=N
     _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
                                         grads.out_type, max_norm, _list_scratch(grads, scratch, dev),
-                                        _dev_ptr(sumsq, dev), _dev_ptr(norm, dev)))
+                                        _scalar_ptr(sumsq, "float64", dev), _scalar_ptr(norm, "float32", dev)))
 
 
 def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:
@@ -578,7 +604,8 @@ def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: 
     GPUs' lists). No counterpart in the reference."""
     _list_on(grads, dev)
     _check(lib().PARALiA_tile_grad_scale(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
-                                         grads.out_type, _dev_ptr(sumsq, dev), max_norm, _dev_ptr(norm, dev)))
+                                         grads.out_type, _scalar_ptr(sumsq, "float64", dev), max_norm,
+                                         _scalar_ptr(norm, "float32", dev)))
 
 
 def malloc(nbytes: int, loc: int) -> int:

@@ -115,3 +115,13 @@ def test_scratch_smaller_than_said_is_refused(pl):
     assert all(_passes(t) for t in _lists(pl, lst, scratch=scratch(n)))
     norm, clip, scale = _lists(pl, lst, scratch=scratch(n - 8))
     assert "scratch holds" in norm and "scratch holds" in clip and _passes(scale)
+
+
+def test_scalars_of_another_type_are_refused(pl):
+    lst = pl.TensorList([Tensor(A, NO_GPU, "torch.float32", 64, 4)])
+    scalar = lambda address, dtype, size, numel=1: Tensor(address, NO_GPU, "torch." + dtype, numel, size)
+    assert all(_passes(t) for t in _lists(pl, lst, sumsq=scalar(D, "float64", 8), norm=scalar(P, "float32", 4, 3)))
+    for norm in (scalar(P, "float64", 8), scalar(P, "bfloat16", 2), scalar(P, "int32", 4), scalar(0, "float32", 4, 0)):
+        assert all("where a float32 is" in t for t in _lists(pl, lst, norm=norm))
+    for sumsq in (scalar(D, "float32", 4, 2), scalar(D, "int64", 8), scalar(0, "float64", 8, 0)):
+        assert all("where a float64 is" in t for t in _lists(pl, lst, sumsq=sumsq))
