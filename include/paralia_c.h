@@ -326,7 +326,8 @@ int PARALiA_tile_ddot_noalloc(int dev, void* stream, int64_t N,
  * (NULL: not kept) is what PARALiA_tile_gemm_act_grad reads. Sums are held in FP32; Z and D
  * are each rounded once from FP32, D from the unrounded Z. As in BLAS, A and B are not read if
  * alpha or K is 0 and C is not read if beta is 0. D may be C (same leading dimension); otherwise
- * no output may share memory with an operand. A dense layer on row-major activations x [tokens, in]
+ * no output, and none of the scratch, may share memory with an operand or one another (views of one
+ * parent that lie between each other's columns do not). A dense layer on row-major activations x [tokens, in]
  * and weights w [out, in] is TransA = 'T', A = w, ldA = in, TransB = 'N', B = x, ldB = in,
  * M = out, N = tokens, K = in, D = y [tokens, out].
  * Any leading dimension and any address that is a multiple of the element size is accepted;
@@ -356,7 +357,8 @@ int PARALiA_tile_gemm_act(int dev, void* stream, int type, char TransA, char Tra
  * the operand that only it needs is not read. The gradient with respect to C is beta * dD. A
  * beta of 1 adds to what earlier calls left (shared weights, several micro-batches). dZ is
  * rounded to `type` before the two products, which take 16-bit operands; dbias is summed in
- * FP32 from the unrounded dZ. No gradient may share memory with another or with an operand.
+ * FP32 from the unrounded dZ. No gradient may share memory with another, with an operand or with the
+ * scratch.
  * `scratch`: PARALiA_tile_gemm_act_grad_scratch_bytes(...) bytes on a 16-byte boundary. That counts room
  * for dZ; a call that makes none (PARALIA_ACT_NONE with dD on 16-byte boundaries, no columns, alpha 0,
  * dbias alone) takes less, and NULL if nothing is left. */

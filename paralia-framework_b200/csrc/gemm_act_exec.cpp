@@ -8,6 +8,7 @@
 
 #include "exec.hpp"
 #include "gemm_act.cuh"
+#include "regions.hpp"
 #include "runtime.hpp"
 
 namespace paralia {
@@ -47,6 +48,19 @@ int check_scratch(const void* scratch, int64_t have, int64_t need) {
 }
 
 bool odd_address(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }
+
+Region matrix(const void* p, int64_t rows, int64_t cols, int64_t ld) { return region(p, rows, cols, ld, 2); }
+
+// Whether one of the n_w written regions shares memory with another of them or with one that is read.
+bool written_overlap(const Region* w, int n_w, const Region* r, int n_r) {
+  for (int i = 0; i < n_w; ++i) {
+    for (int j = i + 1; j < n_w; ++j)
+      if (regions_overlap(w[i], w[j])) return true;
+    for (int j = 0; j < n_r; ++j)
+      if (regions_overlap(w[i], r[j])) return true;
+  }
+  return false;
+}
 
 }  // namespace
 
@@ -96,13 +110,22 @@ int exec_tile_gemm_act(int dev, void* stream, int type, char TransA, char TransB
   if (!D || (product && (!A || !B)) || (beta != 0.0f && !C)) return fail(PARALIA_ERR_INVALID_ARG, "NULL operand");
   if (odd_address(A) || odd_address(B) || odd_address(C) || odd_address(D) || odd_address(bias) || odd_address(pre))
     return fail(PARALIA_ERR_INVALID_ARG, "operand address is not a multiple of the element size");
-  if (D == A || D == B || D == pre || D == bias || (pre && (pre == A || pre == B || pre == bias)) ||
-      (beta != 0.0f && (pre == C || (D == C && ldD != ldC))))
-    return fail(PARALIA_ERR_INVALID_ARG, "an output may share memory with no operand, but D with C at the same leading dimension");
   OperandCopies copies = {GA_COPY_NONE, GA_COPY_NONE, 0, 0};
   if (product) copies = operand_copies(M, N, K, is_trans(TransA), is_trans(TransB), A, ldA, B, ldB);
   if (copies.needed > 0) PL_TRY(check_scratch(scratch, scratch_bytes, copies.needed));
   const int64_t room = scratch && !(reinterpret_cast<uintptr_t>(scratch) & 15) ? scratch_bytes : 0;
+  {
+    const bool ta = is_trans(TransA), tb = is_trans(TransB);
+    // D may be C; a tile of C is read before the same tile of D is written
+    const bool in_place = beta != 0.0f && D == C && (ldD == ldC || N == 1);
+    const int64_t used = room >= copies.bytes ? copies.bytes : copies.needed;
+    const Region w[] = {matrix(D, M, N, ldD), matrix(pre, M, N, ldPre), region(scratch, used, 1, used, 1)};
+    const Region r[] = {matrix(A, ta ? K : M, ta ? M : K, ldA), matrix(B, tb ? N : K, tb ? K : N, ldB),
+                        matrix(bias, M, 1, M), matrix(beta != 0.0f && !in_place ? C : nullptr, M, N, ldC)};
+    if (written_overlap(w, 3, r, 4))
+      return fail(PARALIA_ERR_INVALID_ARG,
+                  "an output or scratch may share memory with no operand, but D with C at the same leading dimension");
+  }
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());
@@ -169,21 +192,27 @@ int exec_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, char T
   if (odd_address(A) || odd_address(B) || odd_address(pre) || odd_address(dD) || odd_address(dA) ||
       odd_address(dB) || odd_address(dbias))
     return fail(PARALIA_ERR_INVALID_ARG, "operand address is not a multiple of the element size");
-  const void* outs[3] = {want_a ? dA : nullptr, want_b ? dB : nullptr, want_bias ? dbias : nullptr};
-  for (int i = 0; i < 3; ++i) {
-    if (!outs[i]) continue;
-    if (outs[i] == A || outs[i] == B || outs[i] == pre || outs[i] == dD || outs[i] == outs[(i + 1) % 3])
-      return fail(PARALIA_ERR_INVALID_ARG, "a gradient may share memory with no operand and no other gradient");
-  }
   // What this call touches of its scratch: nothing without a product; without an activation dZ is dD, in
   // place unless it is to be copied.
   const GradScratch g = grad_scratch(M, N, K, ta, tb, A, ldA, B, ldB);
   const bool products = entries && K > 0 && alpha != 0.0f && (want_a || want_b);
   const int64_t room = scratch && !(reinterpret_cast<uintptr_t>(scratch) & 15) ? scratch_bytes : 0;
   const GemmActCopy copy_z = uses_pre ? GA_COPY_NEEDED : gemm_act_operand_copy(dD, lddD, M, N, K);
-  const bool need_z = products && (copy_z == GA_COPY_NEEDED || (copy_z == GA_COPY_PAYS && room >= g.z_bytes + g.copies.needed));
+  const bool need_z =
+      products && (copy_z == GA_COPY_NEEDED || (copy_z == GA_COPY_PAYS && room >= g.z_bytes + g.copies.needed));
   const int64_t z_bytes = need_z ? g.z_bytes : 0, needed = products ? z_bytes + g.copies.needed : 0;
   if (needed > 0) PL_TRY(check_scratch(scratch, scratch_bytes, needed));
+  const bool every_copy = room - z_bytes >= g.copies.bytes;
+  const int64_t used = !products ? 0 : z_bytes + (every_copy ? g.copies.bytes : g.copies.needed);
+  {
+    const Region w[] = {matrix(want_a ? dA : nullptr, ta ? K : M, ta ? M : K, lddA),
+                        matrix(want_b ? dB : nullptr, tb ? N : K, tb ? K : N, lddB),
+                        matrix(want_bias ? dbias : nullptr, M, 1, M), region(scratch, used, 1, used, 1)};
+    const Region r[] = {matrix(A, ta ? K : M, ta ? M : K, ldA), matrix(B, tb ? N : K, tb ? K : N, ldB),
+                        matrix(uses_pre ? pre : nullptr, M, N, ldPre), matrix(dD, M, N, lddD)};
+    if (written_overlap(w, 4, r, 4))
+      return fail(PARALIA_ERR_INVALID_ARG, "a gradient or scratch may share memory with no operand and no other gradient");
+  }
   DeviceGuard guard;
   Runtime& rt = Runtime::get();
   PL_TRY(rt.init());

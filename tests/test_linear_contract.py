@@ -125,3 +125,67 @@ def test_scalars_of_another_type_are_refused(pl):
         assert all("where a float32 is" in t for t in _lists(pl, lst, norm=norm))
     for sumsq in (scalar(D, "float32", 4, 2), scalar(D, "int64", 8), scalar(0, "float64", 8, 0)):
         assert all("where a float64 is" in t for t in _lists(pl, lst, sumsq=sumsq))
+
+
+SHARES = "may share memory"
+
+
+@pytest.mark.parametrize("kw,refused", [
+    # the last byte of one is the first of the other, and one element further none is shared
+    (dict(D=A + 2 * 64 * 16 - 2), True), (dict(D=A + 2 * 64 * 16), False),
+    (dict(A=D + 2 * 64 * 32 - 2), True), (dict(A=D + 2 * 64 * 32), False),
+    (dict(B=D + 100), True), (dict(Cm=D + 2), True), (dict(Cm=D), False), (dict(Cm=D, ldC=72), True),
+    (dict(Cm=D, N=1, ldC=72), False), (dict(bias=D + 126), True), (dict(bias=D + 2 * 64 * 32), False),
+    (dict(pre=D + 2 * 64 * 32 - 2), True), (dict(pre=D + 2 * 64 * 32), False), (dict(pre=CC + 64), True),
+    (dict(beta=0.0, Cm=D + 2), False),                                      # C is not read
+    # one parent of 200 rows: D, pre and C in rows of their own
+    (dict(D=D, ldD=200, pre=D + 128, ldPre=200, Cm=D + 256, ldC=200), False),
+    (dict(D=D, ldD=200, pre=D + 126, ldPre=200), True), (dict(D=D + 128, ldD=200, pre=D, ldPre=200), False),
+    (dict(D=D + 128, ldD=200, pre=D + 2, ldPre=200), True),
+    # columns of the parent taken apart: rows 136 to 199 of a column, rows 0 to 63 of the next
+    (dict(D=D + 272, ldD=200, pre=D + 400, ldPre=200), False), (dict(D=D + 272, ldD=200, pre=D + 398, ldPre=200), True),
+    # two strides in one range: D has bytes 0 to 127 of every 800; pre at 400 k + 128, + 272 (up to 400 and 800), + 336 (736
+    # to 863), at 402 k + 128 (never beyond 718 of 800) and at 434 k + 128 (698 to 825 for k = 5)
+    (dict(D=D, ldD=400, pre=D + 128, ldPre=200), False), (dict(D=D, ldD=400, pre=D + 272, ldPre=200), False),
+    (dict(D=D, ldD=400, pre=D + 336, ldPre=200), True), (dict(D=D, ldD=400, pre=D + 128, ldPre=201), False),
+    (dict(D=D, ldD=400, pre=D + 128, ldPre=217), True), (dict(pre=D, ldPre=400, D=D + 128, ldD=217), True),
+    # scratch: columns of A off the grid, 64 of 16 elements, copied
+    (dict(A=A + 2, scratch=D + 2 * 64 * 32 - 16), True), (dict(A=A + 2, scratch=D + 2 * 64 * 32), False),
+    (dict(A=A + 2, scratch=D - 2048), False), (dict(A=A + 2, scratch=D - 2032), True), (dict(scratch=D), False),
+])
+def test_outputs_that_overlap_operands(pl, kw, refused):
+    text = _forward(pl, **kw)
+    assert (SHARES in text) if refused else _passes(text), text
+
+
+@pytest.mark.parametrize("kw,refused", [
+    (dict(dA=A + 2 * 64 * 16 - 2), True), (dict(dA=A + 2 * 64 * 16), False), (dict(dB=DA + 32), True),
+    (dict(dB=DA + 2 * 64 * 16), False), (dict(dbias=DA + 2), True), (dict(dbias=DB + 2 * 16 * 32 - 2), True),
+    (dict(dbias=D + 4000), True), (dict(dbias=P + 4000), True), (dict(dA=P - 2), True),
+    (dict(dA=P - 2, act=0), False), (dict(dA=P, act=0), False),            # without an activation pre is not read
+    (dict(dA=DA, lddA=32, dB=DA + 32, lddB=32), False),                    # side by side in one parent
+    (dict(dA=S + 4096), False), (dict(dA=S + 4094), True), (dict(dD=S + 64), True), (dict(act=0, dD=S), False),
+    (dict(dbias=S, dA=None, dB=None), False),                              # nothing of the scratch is touched
+])
+def test_gradients_that_overlap(pl, kw, refused):
+    text = _grad(pl, **kw)
+    assert (SHARES in text) if refused else _passes(text), text
+
+
+def test_overlaps_of_random_matrices(pl):
+    """Three matrices in a range of 700 elements, their elements counted one by one."""
+    import random
+    rng = random.Random(6)
+    seen = {True: 0, False: 0}
+    for _ in range(3000):
+        M, N = rng.randint(1, 12), rng.randint(1, 12)
+        m = [(rng.randrange(0, 700), M + rng.choice((0, 0, rng.randrange(60)))) for _ in range(3)]
+        cells = [{at + i + j * ld for j in range(N) for i in range(M)} for at, ld in m]
+        d, p, c = cells
+        in_place = m[0] == m[2] or N == 1 and m[0][0] == m[2][0]
+        shared = bool(d & p or p & c or (d & c and not in_place))
+        text = _forward(pl, M=M, N=N, A=A, B=B, bias=0, scratch=0, scratch_bytes=0, D=D + 2 * m[0][0], ldD=m[0][1],
+                        pre=D + 2 * m[1][0], ldPre=m[1][1], Cm=D + 2 * m[2][0], ldC=m[2][1])
+        assert (SHARES in text) == shared and _passes(text) != shared, (M, N, m, text)
+        seen[shared] += 1
+    assert min(seen.values()) > 300
