@@ -377,7 +377,9 @@ int PARALiA_tile_gemm_act_grad(int dev, void* stream, int type, char TransA, cha
  * PARALIA_BF16, mixed as they come) at device addresses g[i]. The arrays g, n, type, out and
  * out_type are host memory and are read during the call. Tensors of size 0 are skipped.
  * `scratch`: device memory of PARALiA_tile_grad_norm_scratch_bytes(count) bytes on an 8-byte
- * boundary. The order of the sums depends on the list alone, so results are bit-reproducible.
+ * boundary. scratch, sumsq and norm may share memory with one another or a tensor in no call. The
+ * order of the sums depends on the list alone (sizes, types and addresses modulo 16 bytes), so results
+ * are bit-reproducible.
  *
  * Global norm: *sumsq <- sum over all elements of g^2, *norm <- its square root (device
  * memory; either may be NULL). Sums are carried in FP64. */

@@ -31,6 +31,7 @@ struct GradList {
   int count;                 // tensors with elements
   GradEntry* entries;        // unit0 counts over the whole list
   int64_t units;
+  uintptr_t lo, hi;          // all tensors and outputs lie between these addresses
 };
 
 // Number of partial sums the norm of a list of `count` tensors may leave at most.

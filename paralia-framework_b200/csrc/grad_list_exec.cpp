@@ -33,6 +33,32 @@ bool ranges_conflict(std::vector<Range>& r) {
   return false;
 }
 
+// Scratch and results stand apart from one another and from every tensor: some blocks still read what
+// another one has written its result over.
+int check_apart(const GradList& l, const void* scratch, int64_t scratch_bytes, const void* sumsq, const void* norm) {
+  const void* p[3] = {scratch, sumsq, norm};
+  const int64_t bytes[3] = {scratch_bytes, (int64_t)sizeof(double), (int64_t)sizeof(float)};
+  Range r[3];
+  for (int i = 0; i < 3; ++i) {
+    r[i].lo = reinterpret_cast<uintptr_t>(p[i]);
+    r[i].hi = p[i] ? r[i].lo + bytes[i] : 0;
+  }
+  auto meet = [](const Range& a, uintptr_t lo, uintptr_t hi) { return a.lo < hi && lo < a.hi; };
+  bool near = false, shared = false;
+  for (int i = 0; i < 3; ++i) {
+    for (int j = i + 1; j < 3; ++j) shared = shared || meet(r[i], r[j].lo, r[j].hi);
+    near = near || meet(r[i], l.lo, l.hi);
+  }
+  for (int t = 0; near && t < l.count; ++t) {
+    const GradEntry& e = l.entries[t];
+    const uintptr_t s = reinterpret_cast<uintptr_t>(e.src), d = reinterpret_cast<uintptr_t>(e.dst);
+    const uintptr_t s_end = s + e.n * type_bytes(e.src_type), d_end = d + e.n * type_bytes(e.dst_type);
+    for (const Range& x : r) shared = shared || meet(x, s, s_end) || meet(x, d, d_end);
+  }
+  if (shared) return fail(PARALIA_ERR_INVALID_ARG, "scratch, sumsq and norm may share memory with nothing");
+  return PARALIA_OK;
+}
+
 // Checks the list and describes its non-empty tensors. out == nullptr: in place.
 int describe(int count, const void* const* g, const int64_t* n, const int32_t* type, void* const* out,
              const int32_t* out_type, bool writes, std::vector<GradEntry>* entries, GradList* l) {
@@ -51,6 +77,8 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
       return fail(PARALIA_ERR_INVALID_ARG, "tensor %d: address is not a multiple of the element size", i);
   }
   l->units = 0;
+  l->lo = UINTPTR_MAX;
+  l->hi = 0;
   entries->reserve(count);
   std::vector<Range> reads_writes;
   if (writes) reads_writes.reserve(2 * (size_t)count);
@@ -66,6 +94,8 @@ int describe(int count, const void* const* g, const int64_t* n, const int32_t* t
     e.head = 0;
     const uintptr_t s = reinterpret_cast<uintptr_t>(e.src), d = reinterpret_cast<uintptr_t>(e.dst);
     const int64_t sb = type_bytes(e.src_type), db = type_bytes(e.dst_type);
+    l->lo = std::min(l->lo, std::min(s, d));
+    l->hi = std::max(l->hi, std::max(s + (uintptr_t)(e.n * sb), d + (uintptr_t)(e.n * db)));
     if (e.dst == e.src && e.dst_type == e.src_type) e.flags |= GL_IN_PLACE;
     // the first element from which groups of eight are aligned, and in dst too if that can be
     for (int h = 7; h >= 0; --h) {
@@ -130,6 +160,7 @@ int exec_tile_grad_norm(int dev, void* stream, int count, const void* const* g, 
   PL_TRY(check_scratch(scratch));
   PL_TRY(check_results(sumsq, norm));
   if (!sumsq && !norm) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq and norm");
+  PL_TRY(check_apart(l, scratch, grad_norm_scratch_bytes(count), sumsq, norm));
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -148,6 +179,7 @@ int exec_tile_grad_clip(int dev, void* stream, int count, const void* const* g, 
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   PL_TRY(check_scratch(scratch));
   PL_TRY(check_results(sumsq, norm));
+  PL_TRY(check_apart(l, scratch, grad_norm_scratch_bytes(count), sumsq, norm));
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -166,6 +198,7 @@ int exec_tile_grad_scale(int dev, void* stream, int count, const void* const* g,
   PL_TRY(describe(count, g, n, type, out, out_type, true, &entries, &l));
   if (!sumsq) return fail(PARALIA_ERR_INVALID_ARG, "NULL sumsq");
   PL_TRY(check_results(sumsq, norm));
+  PL_TRY(check_apart(l, nullptr, 0, sumsq, norm));
   DeviceGuard guard;
   PL_TRY(enter(dev, stream));
   // one partial sum is only read

@@ -189,3 +189,29 @@ def test_overlaps_of_random_matrices(pl):
         assert (SHARES in text) == shared and _passes(text) != shared, (M, N, m, text)
         seen[shared] += 1
     assert min(seen.values()) > 300
+
+
+def test_results_and_scratch_of_lists_stand_apart(pl):
+    f32 = lambda address, numel=64: Tensor(address, NO_GPU, "torch.float32", numel, 4)
+    lists = [pl.TensorList([f32(A), f32(B)]), pl.TensorList([f32(A), f32(CC, 0), f32(B)], [f32(DA), f32(CC, 0), f32(DB)])]
+    text = "share memory with nothing"
+    for k, lst in enumerate(lists):
+        n = pl.tile_grad_norm_scratch_bytes(lst)
+        assert all(_passes(t) for t in _lists(pl, lst))
+        # norm inside sumsq, in either half: blocks that read the sum would see the norm
+        for norm in (D, D + 4):
+            assert all(text in t for t in _lists(pl, lst, norm=norm))
+        assert all(_passes(t) for t in _lists(pl, lst, norm=D + 8)) and all(_passes(t) for t in _lists(pl, lst, norm=D - 4))
+        # a result in the scratch or behind it
+        for sumsq, bad in ((S, True), (S + n - 8, True), (S + n, False), (S - 8, False)):
+            got = _lists(pl, lst, sumsq=sumsq)
+            assert [text in t for t in got] == [bad, bad, False] and _passes(got[2])
+        # over a tensor, in its last element and behind it
+        for norm, bad in ((A, True), (B + 252, True), (B + 256, False), (A - 4, False)):
+            assert all((text in t) == bad and _passes(t) != bad for t in _lists(pl, lst, norm=norm)), (k, norm)
+        for sumsq, bad in ((A + 248, True), (A + 256, False)):
+            assert all((text in t) == bad for t in _lists(pl, lst, sumsq=sumsq)), (k, sumsq)
+        for scratch, bad in ((B + 248, True), (B + 256, False), (A - n + 8, True), (A - n, False)):
+            assert [text in t for t in _lists(pl, lst, scratch=scratch)] == [bad, bad, False], (k, scratch)
+    for at, bad in ((DA + 252, True), (DB + 256, False)):     # an output: not where only the tensors are read
+        assert [text in t for t in _lists(pl, lists[1], norm=at)] == [False, bad, bad], at
