@@ -245,26 +245,32 @@ def _ptr(x) -> int:
 
 def _dev_ptr(x, dev=None) -> int:
     """Address of an operand of the mixed-precision routines, which take memory of GPU ``dev`` only (None: of any GPU)."""
-    if x is None or isinstance(x, int):
-        return x or 0
+    if x is None:
+        return 0
+    if type(x) is int:
+        return x
     try:
         at = x.get_device()
     except AttributeError:
+        if isinstance(x, int):
+            return x
         at = -1
-    if at != dev or at < 0:
-        if at < 0:
-            raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
-        if dev is not None:
-            raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is on GPU {at}, the call is for GPU {dev}")
+    if at != dev:
+        _refuse_place(x, at, dev)
     return x.data_ptr()
+
+
+def _refuse_place(x, at, dev) -> None:
+    if at < 0:
+        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is not in GPU memory")
+    if dev is not None:
+        raise ParaliaError(ERR_INVALID_ARG, f"operand {type(x).__name__} is on GPU {at}, the call is for GPU {dev}")
 
 
 def _scratch_ptr(x, nbytes, dev) -> int:
     """Address of scratch of which a call may use ``nbytes``; a tensor has to hold as many."""
-    if x is None or isinstance(x, int):
-        return x or 0
     at = _dev_ptr(x, dev)
-    if x.nbytes < nbytes:
+    if x is not None and not isinstance(x, int) and x.nbytes < nbytes:
         raise ParaliaError(ERR_INVALID_ARG, f"scratch holds {x.nbytes} bytes, {nbytes} are to be used")
     return at
 
@@ -512,11 +518,12 @@ def _dtype_name(x) -> str:
 
 def _scalar_ptr(x, dtype: str, dev) -> int:
     """Address of a device scalar that a list routine reads or writes as ``dtype``."""
-    if x is None or isinstance(x, int):
-        return x or 0
+    if x is None:
+        return 0
     at = _dev_ptr(x, dev)
-    if _dtype_name(x) != dtype or x.nbytes == 0:
-        raise ParaliaError(ERR_INVALID_ARG, f"{x.nbytes} bytes of {_dtype_name(x)} where a {dtype} is read or written")
+    if not isinstance(x, int) and (_DTYPE_NAMES.get(x.dtype) != dtype or x.nbytes == 0):
+        if _dtype_name(x) != dtype or x.nbytes == 0:      # not a type seen for the first time
+            raise ParaliaError(ERR_INVALID_ARG, f"{x.nbytes} bytes of {_dtype_name(x)} where a {dtype} is read or written")
     return at
 
 
@@ -563,18 +570,18 @@ class TensorList:
         self.out_type = None if self.out is None else (_i32 * n)(*[_type_of(t) for t in self.out])
 
 
-def _list_on(grads, dev) -> None:
-    at = getattr(grads, "dev", None)
-    if at != dev and at is not None:
-        raise ParaliaError(ERR_INVALID_ARG, f"the list is on GPU {at}, the call is for GPU {dev}")
-
-
 def _list_scratch(grads, scratch, dev) -> int:
     if scratch is None or isinstance(scratch, int):
         return scratch or 0
-    if grads.scratch_bytes is None:
-        grads.scratch_bytes = tile_grad_norm_scratch_bytes(grads)
-    return _scratch_ptr(scratch, grads.scratch_bytes, dev)
+    need = grads.scratch_bytes
+    if need is None:
+        need = grads.scratch_bytes = tile_grad_norm_scratch_bytes(grads)
+    return _scratch_ptr(scratch, need, dev)
+
+
+def _refuse_list(grads, dev) -> None:
+    if grads.dev is not None:
+        raise ParaliaError(ERR_INVALID_ARG, f"the list is on GPU {grads.dev}, the call is for GPU {dev}")
 
 
 def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
@@ -584,7 +591,8 @@ def tile_grad_norm_scratch_bytes(grads: TensorList) -> int:
 def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of a list of tensors: ``norm`` (float32) and ``sumsq`` (float64, its square) are device
     scalars, either may be None. No counterpart in the reference."""
-    _list_on(grads, dev)
+    if getattr(grads, "dev", dev) != dev:
+        _refuse_list(grads, dev)
     _check(lib().PARALiA_tile_grad_norm(dev, stream, grads.count, grads.g, grads.n, grads.type,
                                         _list_scratch(grads, scratch, dev), _scalar_ptr(sumsq, "float64", dev),
                                         _scalar_ptr(norm, "float32", dev)))
@@ -593,7 +601,8 @@ def tile_grad_norm(dev, grads: TensorList, scratch, norm=None, sumsq=None, strea
 def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=None, stream: int = 0) -> None:
     """Global norm of the list, then every tensor times ``max_norm / norm`` where that is below 1, in place or
     to the list's ``out``. No counterpart in the reference."""
-    _list_on(grads, dev)
+    if getattr(grads, "dev", dev) != dev:
+        _refuse_list(grads, dev)
     _check(lib().PARALiA_tile_grad_clip(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
                                         grads.out_type, max_norm, _list_scratch(grads, scratch, dev),
                                         _scalar_ptr(sumsq, "float64", dev), _scalar_ptr(norm, "float32", dev)))
@@ -602,7 +611,8 @@ def tile_grad_clip(dev, grads: TensorList, max_norm, scratch, norm=None, sumsq=N
 def tile_grad_scale(dev, grads: TensorList, sumsq, max_norm, norm=None, stream: int = 0) -> None:
     """The scaling half of ``tile_grad_clip`` from a squared norm in device memory (the sum over several
     GPUs' lists). No counterpart in the reference."""
-    _list_on(grads, dev)
+    if getattr(grads, "dev", dev) != dev:
+        _refuse_list(grads, dev)
     _check(lib().PARALiA_tile_grad_scale(dev, stream, grads.count, grads.g, grads.n, grads.type, grads.g_out,
                                          grads.out_type, _scalar_ptr(sumsq, "float64", dev), max_norm,
                                          _scalar_ptr(norm, "float32", dev)))
