@@ -373,10 +373,19 @@ __device__ __forceinline__ void ga_finish(const GaProb& a, int64_t r, int64_t q0
   });
 }
 
+// The first `count` of eight packed elements, one by one.
+__device__ __forceinline__ void ga_store_some(uint16_t* p, const uint32_t (&v)[4], int count) {
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < count) p[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+}
+
 // One warp's share of a tile (QC): 32 columns of D, `cols` rows from q on, a multiple of 64. Once Z has
 // been made of the sums of 16 rows, the next 16 are fetched under the rest of the work on these. 64
 // rows at a time leave through this warp's staging buffer (128-byte lines, swizzled as the tensor map
-// says) by TMA: whole lines, edges clipped by the map, the store under the next arithmetic. The loop
+// says) by TMA: whole lines, edges clipped by the map, the store under the next arithmetic. A TMA store
+// writes whole groups of 16 bytes, also where the matrix ends inside one: the map ends with the last whole
+// group, and the one to seven rows behind it are stored one by one. The loop
 // is not unrolled: with ten variants and eight warps out of step the instruction cache is what an
 // unrolled one waits for (8192 x 8192 x 1024 with tanh-GELU: 174 us unrolled by four).
 template <int ACT, bool bf>
@@ -388,6 +397,8 @@ __device__ __forceinline__ void ga_staged_tile(const GaProb& a, const CUtensorMa
   const int left = a.M - q;
   const int last = left >= cols ? cols : (left + 63) / 64 * 64;        // 64 rows of which none exists are left out
   if (last <= 0) return;
+  const int whole = a.M & ~7;                                          // rows that leave by TMA
+  const int rest = r_first + lane < a.N ? a.M - whole : 0;             // rows of this lane's column that do not
   uint32_t v[16];
   uint4 c0 = ga_load_c8(a, q, n), c1 = ga_load_c8(a, (int64_t)q + 8, n);
   uint4 b0 = ga_load_bias8(a, q), b1 = ga_load_bias8(a, (int64_t)q + 8);
@@ -415,20 +426,27 @@ __device__ __forceinline__ void ga_staged_tile(const GaProb& a, const CUtensorMa
     }
     uint32_t o[4];
     const uint32_t to0 = row + (((at & 63) >> 3) ^ (lane & 7)) * 16, to1 = row + ((((at & 63) >> 3) + 1) ^ (lane & 7)) * 16;
+    const bool end0 = q + at == whole, end1 = q + at + 8 == whole;
+    uint16_t* const tail = static_cast<uint16_t*>(a.D) + whole + n * a.ldD;
     ga_d8<ACT, bf>(a, z, cx0, o);
     st_shared16(to0, o);
+    if (end0) ga_store_some(tail, o, rest);
     ga_d8<ACT, bf>(a, z + 8, cx1, o);
     st_shared16(to1, o);
+    if (end1) ga_store_some(tail, o, rest);
     if (a.pre) {
+      uint16_t* const tail_pre = static_cast<uint16_t*>(a.pre) + whole + n * a.ldPre;
       ga_pack8<bf>(z, o);
       st_shared16(to0 + 4096, o);
+      if (end0) ga_store_some(tail_pre, o, rest);
       ga_pack8<bf>(z + 8, o);
       st_shared16(to1 + 4096, o);
+      if (end1) ga_store_some(tail_pre, o, rest);
     }
     if ((at & 63) == 48) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0 && r_first < a.N) {
+      if (lane == 0 && r_first < a.N && q + at - 48 < whole) {
         ga_store(map_d, out, q + at - 48, r_first);
         if (a.pre) ga_store(map_pre, out + 4096, q + at - 48, r_first);
         ga_store_commit();
@@ -1143,11 +1161,13 @@ int ga_launch_products(const GemmActProblem* ps, int n, const GaPlan& v, bool ve
                    v.qc ? yrows : xrows, v.qc ? &a.y_mn : &a.x_mn));
     PL_TRY(operand(v.qc ? &maps.x[i] : &maps.y[i], p.B, p.ldB, p.tb ? p.N : p.K, p.tb ? p.K : p.N, b_k,
                    v.qc ? xrows : yrows, v.qc ? &a.x_mn : &a.y_mn));
-    if (g.stage_out) {
+    if (g.stage_out && p.M >= 8) {
+      // whole groups of eight rows; the kernel stores what is behind them
       // (the leading dimension of a single column has no meaning and any value)
       const int64_t ld1 = ((int64_t)p.M + 7) / 8 * 8, ldD = p.N > 1 ? p.ldD : ld1, ldPre = p.N > 1 ? p.ldPre : ld1;
-      PL_TRY(make_tensor_map(&maps.d[i], p.D, 2, p.M, p.N, 1, ldD * 2, (uint64_t)ldD * p.N * 2, 64, 32));
-      if (p.pre) PL_TRY(make_tensor_map(&maps.pre, p.pre, 2, p.M, p.N, 1, ldPre * 2, (uint64_t)ldPre * p.N * 2, 64, 32));
+      const uint64_t whole = p.M & ~7;
+      PL_TRY(make_tensor_map(&maps.d[i], p.D, 2, whole, p.N, 1, ldD * 2, (uint64_t)ldD * p.N * 2, 64, 32));
+      if (p.pre) PL_TRY(make_tensor_map(&maps.pre, p.pre, 2, whole, p.N, 1, ldPre * 2, (uint64_t)ldPre * p.N * 2, 64, 32));
     }
     if (i == 0) g.tiles0 = (int32_t)tiles;
   }
