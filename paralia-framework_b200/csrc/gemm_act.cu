@@ -1214,7 +1214,9 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
       ld = ld_copy;   // of no meaning, but TMA wants a multiple of 16 bytes
     }
   };
-  auto vec16 = [](const void* q, int64_t ld) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0 && (ld & 7) == 0; };
+  // Results leave as 16-byte groups only if everything that is read or written beside them can: D, C, pre and
+  // the bias, of every product of the call. One of them off the grid, the bias too, leaves the variants with
+  // two-byte stores.
   bool vec = true;
   for (int i = 0; i < n; ++i) {
     GemmActProblem& p = ps[i];
@@ -1237,8 +1239,9 @@ int launch_gemm_act(const GemmActProblem* problems, int count, void* scratch, in
 
 cudaError_t launch_act_grad(const ActGradProblem& p, cudaStream_t stream) {
   if (p.M == 0) return cudaSuccess;
-  // a function of the sizes alone, so that the order of the row sums is too: as many blocks to a
-  // cluster as there are columns for, eight at most
+  // a function of the sizes alone; with that of the two loads, the order of the row sums depends on the sizes
+  // and on whether rows come as 16-byte groups. As many blocks to a cluster as there are columns for,
+  // eight at most
   int parts = 1;
   while (parts < 8 && p.N >= parts * AG_COLS) parts *= 2;
   const int64_t grid = (p.M + AG_ROWS - 1) / AG_ROWS * (int64_t)parts;

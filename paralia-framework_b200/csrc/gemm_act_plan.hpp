@@ -26,6 +26,9 @@ struct GaPlan {
 // to 3100 timings of 134 shapes (1 to 2048 columns, 300 to 16384 rows, k 256 to 10240) with every
 // variant that fits them: the variant it picks is 1.2 % slower than the fastest in the mean, 30 % at
 // worst (1024 x 37 x 1024, 6.9 against 5.3 us).
+// It knows nothing of columns off 32-byte sectors that are read in place (2888 x 656 x 9320 takes 128 x 128
+// tiles, 68 us, where CTA pairs take 58). k is split for tiles of one CTA only; the sum over a cluster is
+// written for those.
 // Shifts and products in place of most divisions: this is host time of every call (thirty variants, 0.22 us; 1.05 with them).
 inline double ga_cost(const GaPlan& v, const int64_t* tiles_of, const int64_t* kblocks, double hbm_bytes, int count) {
   const int log_split = v.split == 1 ? 0 : v.split == 2 ? 1 : v.split == 4 ? 2 : 3;

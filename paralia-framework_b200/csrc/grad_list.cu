@@ -6,10 +6,10 @@
 // calls, capturable). It is cut into units of 2048 elements and block b of G takes the b-th of G
 // equal runs of units, so what a block has of one tensor is one contiguous span (chunks dealt out
 // in turn, with a search for the tensor of each, read 2 GB of BF16 in 365 us; this takes 302, 6.6
-// TB/s). The order of every sum is a function of the list alone.
+// TB/s). The order of every sum is a function of the list alone: sizes, types, addresses modulo 16 bytes.
 //
 // Squares: of FP32 elements they are summed in FP64 throughout (a conversion and an FMA an
-// element, which the FP64 pipe keeps up with at HBM speed). Of 16-bit elements the eight of
+// element, which the FP64 pipe keeps up with at HBM speed: 256 Mi elements 161 us, 6.67 TB/s). Of 16-bit elements the eight of
 // one 16-byte load are summed in FP32 (their squares are exact there) and the sum goes to
 // FP64: one conversion for eight elements instead of eight, at a relative error of a few
 // 2^-24 per group of eight. Where such a sum leaves the range in which FP32 is that exact, the group is
@@ -412,7 +412,8 @@ cudaError_t launch_scale(const GradTable<CAP>& t, const double* partials, int us
   const int chunk = std::max(1, std::min(GL_CHUNK, t.units / GL_NORM_BLOCKS));
   const int grid = (t.units + chunk - 1) / chunk;
   // one pair of types for the whole list, as most lists have it, gets a kernel of its own: a third
-  // fewer registers than the one that looks at every tensor's
+  // fewer registers than the one that looks at every tensor's. FP16 to BF16 and back share that one, which
+  // costs them nothing that shows: 256 Mi elements take 156 and 157 us, BF16 to BF16 157
   const int src = t.e[0].src_type, dst = t.e[0].dst_type;
   bool same = true;
   for (int i = 1; i < t.count && same; ++i) same = t.e[i].src_type == src && t.e[i].dst_type == dst;

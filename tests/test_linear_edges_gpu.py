@@ -85,3 +85,15 @@ def test_gradient_without_inner_dimension(pl):
     torch.cuda.synchronize()
     pl.tile_status(0)
     assert bool((db == N / 2).all())
+
+
+@pytest.mark.parametrize("cut", [1, 3, 7])
+@pytest.mark.parametrize("dims", [(8, 2000, 128), (8, 15000, 136), (16, 300, 2000), (72, 4440, 64), (2056, 40, 64)])
+def test_few_rows_that_end_inside_a_group(pl, cut, dims):
+    # no whole group of eight rows, or a last one by itself in a tile; the outer products of the gradient likewise
+    d, t = _mods()
+    M, N, K = dims[0] - cut, dims[1], dims[2]
+    for act in ("none", "relu"):
+        t._forward(pl, d, "bf16", "T", "N", M, N, K, pad=cut, ints=True, act=act, bias=True, beta=1.0, pre=True)
+    t._grad(pl, d, "fp16", "N", "T", M, N, K, pad=cut, ints=True, act="relu", betas=(1.0, 1.0, 1.0))
+    t._grad(pl, d, "bf16", "T", "N", M, N, K - cut, pad=cut, ints=True)
